@@ -1,0 +1,82 @@
+// What the kernels of attention to an encoder's states share: their arguments, a row's range of positions, and a row's exact sums.
+//   out[t, h] = sum_j softmax_j(scale q[t, h] . k[j, h / G]) v[j, h / G]   over lo_t <= j < min(hi_t, len_r),   0 where that range is empty;
+// r is token t's request, len_r the length of its source, [lo_t, hi_t) its span (all positions without spans).  Keys and values lie in pages
+// [page][kv head][position in page][d], looked up in the request's row of the block table.
+// The rows that share a kv head's keys are (token, query head of the group) pairs, token by token: row i of a request is token i / G, head i % G.
+#pragma once
+#include "common.cuh"
+#include "launch.cuh"
+
+struct CrossArgs {
+    const void* q;                 // [T] rows q_stride elements apart: H heads of d
+    const void* k_cache;
+    const void* v_cache;
+    void* out;                     // [T, H * d]
+    const int* block_table;        // [R, max_pages]
+    const int* lens;               // [R]
+    const int* cu_tokens;          // [R + 1]
+    const int* spans;              // [T, 2] or null
+    long long q_stride;
+    int max_pages, K, G, d, page_shift;
+    float scale;
+};
+
+// The positions token t of a request sees, cut to its source; (0, 0) where there are none.
+__device__ __forceinline__ int2 cross_range(const CrossArgs& a, int t, int len) {
+    int lo = 0, hi = len;
+    if (a.spans != nullptr) { lo = max(0, a.spans[2 * (size_t)t]); hi = min(len, a.spans[2 * (size_t)t + 1]); }
+    return hi > lo ? make_int2(lo, hi) : make_int2(0, 0);
+}
+
+template <typename T>
+__device__ __forceinline__ const T* cross_row(const CrossArgs& a, const void* cache, const int* table, int kh, int key) {
+    const size_t page = (size_t)table[key >> a.page_shift];
+    return (const T*)cache + (((page * a.K + kh) << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * a.d;
+}
+
+// One row's result from its own range alone, by one warp: where a result is not finite, a value that this row does not see may be what is not
+// (0 * infinity in a tile shared with rows that do see it).  All 32 lanes call it.
+template <typename T>
+__device__ __noinline__ void cross_row_alone(const CrossArgs& a, int t, int head, int request, int2 range) {
+    const int lane = threadIdx.x & 31, kh = head / a.G;
+    const T* q = (const T*)a.q + (size_t)t * a.q_stride + (size_t)head * a.d;
+    const int* table = a.block_table + (size_t)request * a.max_pages;
+    T* out = (T*)a.out + ((size_t)t * a.K * a.G + head) * a.d;
+    const float sl2 = a.scale * 1.4426950408889634f;
+    auto score = [&](int key) {
+        const T* k = cross_row<T>(a, a.k_cache, table, kh, key);
+        float s = 0.0f;
+        for (int i = 0; i < a.d; ++i) s = fmaf(to_f32(q[i]), to_f32(k[i]), s);
+        return s * sl2;
+    };
+    float m = -INFINITY;
+    for (int key = range.x + lane; key < range.y; key += 32) { const float s = score(key); m = s != s ? s : fmaxf(m, s); if (m != m) break; }
+    const bool odd = __any_sync(0xffffffffu, m != m);
+    m = odd ? __int_as_float(0x7fc00000) : warp_max(m);
+    if (m == -INFINITY) m = 0.0f;
+    for (int c0 = 0; c0 < a.d; c0 += 32) {
+        const int c = c0 + lane;
+        float l = 0.0f, acc = 0.0f;
+        for (int key0 = range.x; key0 < range.y; key0 += 32) {
+            const float p = key0 + lane < range.y ? exp2f(score(key0 + lane) - m) : 0.0f;
+            for (int j = 0; j < 32 && key0 + j < range.y; ++j) {
+                const float pj = __shfl_sync(0xffffffffu, p, j);
+                l += pj;
+                if (c < a.d) acc = fmaf(pj, to_f32(cross_row<T>(a, a.v_cache, table, kh, key0 + j)[c]), acc);
+            }
+        }
+        if (c < a.d) out[c] = from_f32<T>(l == 0.0f ? 0.0f : acc / l);
+    }
+}
+
+// A float from the shared memory of CTA `rank` of this cluster, at the address `addr` has in this CTA.
+__device__ __forceinline__ float cross_peer(uint32_t addr, int rank) {
+    uint32_t remote;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cross_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}

@@ -1,0 +1,181 @@
+// A step's page bookkeeping on the device, from the requests' lengths before and after it (one launch, nothing read back):
+//   request r holds pages(before[r]) pages and needs pages(after[r]) = ceil(after[r] / page_size).  Grown requests take pages, shrunk or
+//   ended ones (after = 0) give theirs back; grown ones bring after - before new tokens.
+//   The pages given back lie on top of the free list, in the order of requests and of their positions; pages are taken from its top in the same order:
+//   take number i is entry pool - 1 - i of that stack, pool = count + given back.
+// With the running sums over requests of new tokens, pages taken and pages given back, every output is worked out by itself: a token finds its
+// request by bisection, its page in the block table or, if that page is one of this step's, in the stack; so there is no order between threads and no
+// atomic, and the results are the same bits in every run.  Reads and writes are disjoint: the free list is read below `count` and written from there on,
+// the block table is read where pages were held and written where they are new.
+// Every block makes the running sums itself (R additions of three numbers: a second launch or a wait between blocks would cost more).
+// Bound by latency: a launch, one round trip for the lengths, the sums' three rounds of shuffles, a bisection in shared memory, one round trip for a page.
+#define MB_LIB "pages"
+#define MB_LIB_ID 40
+#include "common.cuh"
+#include "launch.cuh"
+
+#define PG_MAX_REQUESTS 16384
+#define PG_LIMIT (1u << 30)        // sums stop here: what a launch can hold is less, and lengths nobody meant cannot wrap around
+
+struct PageStep {
+    const int* before;             // [R]
+    const int* after;              // [R]
+    int* table;                    // [R, columns]
+    int* free;                     // [free_size], `count` of them filled
+    const int* count;              // [1]
+    int* left;                     // [2]: pages in the free list after the step; 0, or why nothing was done
+    int* cu;                       // [R + 1]
+    int* req;                      // [room] each
+    int* pos;
+    int* slots;
+    int R, columns, free_size, shift, room;
+};
+
+__device__ __forceinline__ unsigned capped(unsigned v) { return v < PG_LIMIT ? v : PG_LIMIT; }
+__device__ __forceinline__ int pages_for(int tokens, int shift) { return (int)(((unsigned)tokens + (1u << shift) - 1u) >> shift); }
+
+// The last r with upto[r] <= x (upto[0] = 0, not decreasing, x < upto[R]).
+__device__ __forceinline__ int owner_of(const unsigned* upto, int R, unsigned x) {
+    int lo = 0, hi = R;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (upto[mid] <= x) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(1024) page_step_kernel(PageStep p) {
+    extern __shared__ unsigned pg_sums[];
+    unsigned* upto_new = pg_sums;                                   // [R + 1] each
+    unsigned* upto_taken = upto_new + p.R + 1;
+    unsigned* upto_back = upto_taken + p.R + 1;
+    __shared__ unsigned warp_total[3][32];
+    PDL_ENTER();
+    p.before = pdl_fresh(p.before); p.after = pdl_fresh(p.after); p.table = pdl_fresh(p.table); p.free = pdl_fresh(p.free); p.count = pdl_fresh(p.count);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
+    const int per = (p.R + threads - 1) / threads, first = min(p.R, tid * per), last = min(p.R, first + per);
+    const int count = p.count[0];
+    unsigned sum[3] = {0u, 0u, 0u};
+    int bad = 0;
+    for (int r = first; r < last; ++r) {
+        const int b = p.before[r], a = p.after[r];
+        if (a < 0 || b < 0) { bad = 1; continue; }
+        const int held = pages_for(b, p.shift), wants = pages_for(a, p.shift);
+        bad |= held > p.columns || wants > p.columns;
+        sum[0] = capped(sum[0] + (unsigned)max(0, min(a - b, (int)PG_LIMIT)));
+        sum[1] = capped(sum[1] + (unsigned)max(0, wants - held));
+        sum[2] = capped(sum[2] + (unsigned)max(0, held - wants));
+    }
+    unsigned upto[3];                                               // of the threads ahead of this one
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        unsigned v = sum[k];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned other = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v = capped(v + other);
+        }
+        if (lane == 31) warp_total[k][warp] = v;
+        const unsigned ahead = __shfl_up_sync(0xffffffffu, v, 1);
+        upto[k] = lane == 0 ? 0u : ahead;
+    }
+    bad = __syncthreads_or(bad);
+    if (!bad) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            unsigned v = lane < (threads >> 5) ? warp_total[k][lane] : 0u;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned other = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v = capped(v + other);
+            }
+            const unsigned ahead = __shfl_sync(0xffffffffu, v, (warp + 31) & 31);
+            if (warp > 0) upto[k] = capped(upto[k] + ahead);
+            if (tid == 0) pg_sums[k * (p.R + 1) + p.R] = 0u;
+        }
+        for (int r = first; r < last; ++r) {
+            const int b = p.before[r], a = p.after[r], held = pages_for(b, p.shift), wants = pages_for(a, p.shift);
+            upto_new[r] = upto[0]; upto_taken[r] = upto[1]; upto_back[r] = upto[2];
+            upto[0] = capped(upto[0] + (unsigned)max(0, min(a - b, (int)PG_LIMIT)));
+            upto[1] = capped(upto[1] + (unsigned)max(0, wants - held));
+            upto[2] = capped(upto[2] + (unsigned)max(0, held - wants));
+            if (r == p.R - 1) { upto_new[p.R] = upto[0]; upto_taken[p.R] = upto[1]; upto_back[p.R] = upto[2]; }
+        }
+    }
+    __syncthreads();
+    unsigned n_new = 0, n_taken = 0, n_back = 0;
+    int status = 3;
+    if (!bad) {
+        n_new = upto_new[p.R]; n_taken = upto_taken[p.R]; n_back = upto_back[p.R];
+        status = n_new > (unsigned)p.room ? 2
+                 : count < 0 || count > p.free_size ? 4
+                 : n_taken > (unsigned)count + n_back ? 1
+                 : (unsigned)count + n_back - n_taken > (unsigned)p.free_size ? 4 : 0;
+    }
+    const int at = blockIdx.x * threads + tid, stride = gridDim.x * threads;
+    if (at == 0) {
+        p.left[0] = status == 0 ? (int)((unsigned)count + n_back - n_taken) : count;
+        p.left[1] = status;
+    }
+    if (status != 0) {
+        for (int r = at; r <= p.R; r += stride) p.cu[r] = 0;
+        for (int t = at; t < p.room; t += stride) { p.req[t] = 0; p.pos[t] = 0; p.slots[t] = -1; }
+        return;
+    }
+    const unsigned pool = (unsigned)count + n_back;
+    // page `i` of the stack: what the free list held, and on top of it what this step gives back
+    auto stacked = [&](unsigned i) -> int {
+        if (i < (unsigned)count) return p.free[i];
+        const unsigned k = i - (unsigned)count;
+        const int r = owner_of(upto_back, p.R, k);
+        return p.table[(size_t)r * p.columns + pages_for(p.after[r], p.shift) + (int)(k - upto_back[r])];
+    };
+    for (int r = at; r <= p.R; r += stride) p.cu[r] = (int)upto_new[r];
+    for (int t = at; t < p.room; t += stride) {
+        int r = 0, position = 0, slot = -1;
+        if ((unsigned)t < n_new) {
+            r = owner_of(upto_new, p.R, (unsigned)t);
+            const int b = p.before[r], held = pages_for(b, p.shift);
+            position = b + (int)((unsigned)t - upto_new[r]);
+            const int column = position >> p.shift;
+            const int page = column < held ? p.table[(size_t)r * p.columns + column] : stacked(pool - 1u - (upto_taken[r] + (unsigned)(column - held)));
+            slot = (page << p.shift) + (position & ((1 << p.shift) - 1));
+        }
+        p.req[t] = r; p.pos[t] = position; p.slots[t] = slot;
+    }
+    for (unsigned i = at; i < n_taken; i += stride) {
+        const int r = owner_of(upto_taken, p.R, i);
+        p.table[(size_t)r * p.columns + pages_for(p.before[r], p.shift) + (int)(i - upto_taken[r])] = stacked(pool - 1u - i);
+    }
+    for (unsigned i = (unsigned)count + at; i + n_taken < pool; i += stride) p.free[i] = stacked(i);
+}
+
+static bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+    return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
+
+// before, after [R], table [R, columns], free [free_size], count [1], left [2], cu [R + 1], req, pos, slots [room]: int32.  page_size: a power of two.
+// left[1]: 0; 1: the free list runs out of pages; 2: more new tokens than `room`; 3: a length is negative or needs more pages than a row of the table
+// has; 4: the free list cannot hold what is given back (or `count` is none of its lengths).  Where it is not 0 nothing is taken or given back.
+MB_API int mb_page_step(const int* before, const int* after, int* table, int* free, const int* count, int* left, int* cu, int* req, int* pos, int* slots,
+                        int R, int columns, int free_size, int page_size, int room, cudaStream_t s) {
+    if (R <= 0 || R > PG_MAX_REQUESTS || columns <= 0 || (long long)R * columns >= PG_LIMIT || free_size < 0 || free_size >= (int)PG_LIMIT || room < 0 ||
+        room >= (int)PG_LIMIT || page_size <= 0 || (page_size & (page_size - 1)) != 0)
+        return MB_ERR_BAD_SIZE;
+    // what every block reads must not be what another has written by then
+    const void* part[] = {before, after, count, table, free, left, cu, req, pos, slots};
+    const size_t n[] = {(size_t)R, (size_t)R, 1, (size_t)R * columns, (size_t)free_size, 2, (size_t)R + 1, (size_t)room, (size_t)room, (size_t)room};
+    for (int i = 0; i < 10; ++i)
+        for (int j = i + 1; j < 10; ++j)
+            if (j >= 3 && overlap(part[i], n[i] * 4, part[j], n[j] * 4)) return MB_ERR_BAD_SIZE;
+    int shift = 0;
+    while ((1 << shift) < page_size) ++shift;
+    const int threads = R <= 256 ? 256 : 1024;
+    const int blocks = max(1, min(148, (room + threads - 1) / threads));
+    const size_t smem = 3 * ((size_t)R + 1) * sizeof(unsigned);
+    static LaunchSmem allowed;
+    const int rc = allowed.allow(page_step_kernel, 3 * (PG_MAX_REQUESTS + 1) * sizeof(unsigned));
+    if (rc != 0) return rc;
+    const PageStep p = {before, after, table, free, count, left, cu, req, pos, slots, R, columns, free_size, shift, room};
+    return launch_kernel(page_step_kernel, dim3(blocks), dim3(threads), smem, s, 0, p);
+}

@@ -166,6 +166,9 @@ LIBRARIES: Dict[str, List[str]] = {
     "mb_layer_norm": ["layer_norm.cu"],
     "mb_delta_rule": ["delta_rule.cu"],
     "mb_gated_linear": ["gated_linear.cu"],
+    "mb_pages": ["pages.cu"],
+    "mb_rope_axes": ["rope_axes.cu"],
+    "mb_attention_cross": ["attention_cross.cu"],
     "mb_host": ["host/cache_core.cpp", "host/scheduler.cpp", "host/sampler.cpp", "host/safetensors.cpp"],
 }
 

@@ -2804,3 +2804,161 @@ def gla_jobs(dtype, d: int, dv: int, rank: int) -> dict:
         name, job = _gla_chunked_job(d, dv)
         jobs[name] = job
     return jobs
+
+
+# ---- a decoder that reads an encoder's states: heads with positions of several axes, the states' pages, attention to them ----
+
+def _on_current_device(*tensors) -> None:
+    """Launches go to the current device's stream: tensors of another device (or of the host) are refused."""
+    here = _current_device() if torch.cuda.is_available() else -1
+    for t in tensors:
+        if t is not None and (here < 0 or t.get_device() != here):
+            raise KernelError(f"marin_b200 kernels run on tensors of the current CUDA device ({'none' if here < 0 else here}); there is no CPU path: got one on {t.device}")
+
+
+def _int32(what: str, *tensors) -> None:
+    for t in tensors:
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise KernelError(f"{what}: expects contiguous int32 tensors, got {t.dtype}")
+
+
+def axis_sections(sections, spread: bool = False) -> list:
+    """Which axis each pair of a head turns with, for ``sections[a]`` pairs of axis ``a``: the axes' pairs one section after another, or, ``spread``,
+    the axes in turn as long as they have pairs left.  (``qk_norm_axes_write`` takes the list as an int32 tensor.)"""
+    left = [int(n) for n in sections]
+    if not left or min(left) < 0:
+        raise ValueError(f"axis_sections: expects the number of pairs of every axis, got {sections}")
+    if not spread:
+        return [a for a, n in enumerate(left) for _ in range(n)]
+    out = []
+    while any(left):
+        for a in range(len(left)):
+            if left[a] > 0:
+                left[a] -= 1
+                out.append(a)
+    return out
+
+
+def qk_norm_axes_write(rows: torch.Tensor, q_out: Optional[torch.Tensor], q_weight, k_weight, eps: float, positions: torch.Tensor, axis_of: torch.Tensor,
+                       inv_freq: Optional[torch.Tensor], rotary_dim: int, interleaved: bool, slot_mapping: Optional[torch.Tensor], k_cache, v_cache, H: int, K: int, d: int,
+                       write_kv: bool = True) -> None:
+    """``qk_norm_rope_write`` with positions of several axes: of a row's ``H`` query, ``K`` key and ``K`` value heads queries and keys are normed (float32
+    weights ``[d]`` or None) and their pairs turned, pair ``i`` by ``positions[axis_of[i], t] * inv_freq[i]`` (``positions`` int32 ``[axes, T]``, ``axis_of`` int32 and
+    ``inv_freq`` float32 ``[rotary_dim / 2]``; the angle in 64 bits); queries go to ``q_out`` ``[T, H * d]``, keys and values into the paged caches at ``slot_mapping``
+    (negative: a padded token, nothing is stored).  ``rows`` ``[T, >= (H + 2 K) * d]`` may be columns of wider rows.  ``H = 0`` (``q_out`` None): an encoder's
+    keys and values alone; ``write_kv=False``: queries alone.  ``axis_of`` is held to the axes there are, places past the caches store nothing."""
+    _on_current_device(rows, q_out, q_weight, k_weight, positions, axis_of, inv_freq, slot_mapping, k_cache, v_cache)
+    if rows.dim() != 2:
+        raise KernelError(f"qk_norm_axes_write: rows are [T, columns], got {tuple(rows.shape)}")
+    T = rows.shape[0]
+    wanted = (H + 2 * K if write_kv else H) * d
+    if rows.shape[1] < wanted or H < 0 or K < 0 or wanted <= 0 or (rows.shape[1] > 1 and rows.stride(1) != 1):
+        raise KernelError(f"qk_norm_axes_write: {tuple(rows.shape)} is not rows of {H} query and {K if write_kv else 0} key and value heads of {d}")
+    if H > 0 and (q_out is None or tuple(q_out.shape) != (T, H * d) or q_out.dtype != rows.dtype or not q_out.is_contiguous()):
+        raise KernelError(f"qk_norm_axes_write: q_out is a contiguous {rows.dtype} tensor [{T}, {H * d}]")
+    for w in (q_weight, k_weight):
+        if w is not None and (w.dtype != torch.float32 or w.numel() != d or not w.is_contiguous()):
+            raise KernelError(f"qk_norm_axes_write: norm weights are float32 [{d}]")
+    if inv_freq is not None:
+        if rotary_dim <= 0 or rotary_dim > d or rotary_dim % 2:
+            raise KernelError(f"qk_norm_axes_write: rotary_dim {rotary_dim} must be even and within the head's {d}")
+        _int32("qk_norm_axes_write", positions, axis_of)
+        if (positions.dim() != 2 or positions.shape[1] != T or positions.shape[0] < 1 or axis_of.numel() != rotary_dim // 2 or inv_freq.numel() != rotary_dim // 2
+                or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous()):
+            raise KernelError(f"qk_norm_axes_write: positions are [axes, {T}], axis_of and inv_freq [{rotary_dim // 2}]")
+    page_size = cache_rows = 0
+    if write_kv:
+        _int32("qk_norm_axes_write", slot_mapping)
+        if (k_cache.dtype != rows.dtype or v_cache.dtype != rows.dtype or k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1] != K or k_cache.shape[3] != d
+                or not k_cache.is_contiguous() or not v_cache.is_contiguous() or slot_mapping.numel() != T):
+            raise KernelError(f"qk_norm_axes_write: caches are contiguous {rows.dtype} [pages, {K}, page_size, {d}] with a slot for each of {T} tokens")
+        page_size = k_cache.shape[2]
+        cache_rows = k_cache.shape[0] * page_size
+    if T == 0:
+        return
+    _cost(2 * T * wanted * rows.element_size() + (_size(positions) if inv_freq is not None else 0), 8.0 * T * wanted)
+    _check(_lib("mb_rope_axes").mb_heads_axes(
+        _ptr(rows), _code(rows), ctypes.c_longlong(rows.stride(0)), _ptr(q_out), _ptr(q_weight), _ptr(k_weight), _c_float(eps), _ptr(positions),
+        _c_int(positions.shape[0] if inv_freq is not None else 0), _ptr(axis_of), _ptr(inv_freq), _c_int(rotary_dim if inv_freq is not None else 0), _c_int(int(interleaved)),
+        _ptr(slot_mapping), _ptr(k_cache), _ptr(v_cache), ctypes.c_longlong(cache_rows), _c_int(page_size), _c_int(T), _c_int(H), _c_int(K), _c_int(d),
+        _c_int(int(write_kv)), _stream()), "qk_norm_axes_write")
+
+
+#: most requests of one ``page_step`` (the running sums over them lie in a block's shared memory)
+PAGE_STEP_REQUESTS = 16384
+
+
+def page_step(before: torch.Tensor, after: torch.Tensor, table: torch.Tensor, free: torch.Tensor, count: torch.Tensor, page_size: int, left: torch.Tensor,
+              cu_tokens: torch.Tensor, req_index: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor) -> None:
+    """A step's bookkeeping on the device (all int32): request ``r`` goes from ``before[r]`` to ``after[r]`` positions.  Requests that grow take pages of
+    ``page_size`` (a power of two) positions into their row of ``table`` ``[R, columns]``, requests that shrink or end (0) give theirs back; pages given back are
+    laid on top of the free list (``free``, of which ``count[0]`` entries are filled) in the order of requests and positions, and pages are taken from its top.
+    ``left`` ``[2]``: the pages then free, and 0.  The new tokens (``after - before`` of them, request by request) get ``cu_tokens`` ``[R + 1]`` and, in buffers of any room,
+    ``req_index``, ``positions`` and ``slots``; the rest of the buffers is 0, 0 and -1 (a padded token).  Rows of ``table`` past what a request holds are
+    left as they were.  ``before``, ``after`` and ``count`` stay: the caller hands in ``after`` and ``left`` next time.
+
+    All or nothing: where ``left[1]`` is 1 (the free list runs out), 2 (more new tokens than the buffers' room), 3 (a length is negative or longer than a row of the
+    table) or 4 (``count`` or what is given back is more than ``free`` holds), no page moves, ``left[0]`` is ``count[0]`` and every token is a padded one."""
+    _on_current_device(before, after, table, free, count, left, cu_tokens, req_index, positions, slots)
+    _int32("page_step", before, after, table, free, count, left, cu_tokens, req_index, positions, slots)
+    R, room = before.numel(), slots.numel()
+    if R < 1 or R > PAGE_STEP_REQUESTS:
+        raise KernelError(f"page_step: 1 to {PAGE_STEP_REQUESTS} requests, got {R}")
+    if (after.numel() != R or table.dim() != 2 or table.shape[0] != R or table.shape[1] < 1 or count.numel() != 1 or left.numel() != 2 or cu_tokens.numel() != R + 1
+            or req_index.numel() != room or positions.numel() != room):
+        raise KernelError(f"page_step: after [{R}], table [{R}, columns], count [1], left [2], cu_tokens [{R + 1}] and buffers of one size are wanted")
+    if page_size < 1 or page_size & (page_size - 1):
+        raise KernelError(f"page_step: page_size {page_size} is no power of two")
+    _cost(4 * (2 * R + R + 1 + 3 * room))
+    _check(_lib("mb_pages").mb_page_step(_ptr(before), _ptr(after), _ptr(table), _ptr(free), _ptr(count), _ptr(left), _ptr(cu_tokens), _ptr(req_index), _ptr(positions),
+                                         _ptr(slots), _c_int(R), _c_int(table.shape[1]), _c_int(free.numel()), _c_int(page_size), _c_int(room), _stream()),
+           "page_step (tensors must not overlap)")
+
+
+class Source:
+    """What a step's requests attend to besides their own cache: an encoder's states in pages.  ``block_table`` int32 ``[R, max_pages]``, ``lens`` int32 ``[R]``
+    (0: a request without a source), ``longest``: no request's source is longer (a number of the host's)."""
+    __slots__ = ("block_table", "lens", "longest")
+
+    def __init__(self, block_table: torch.Tensor, lens: torch.Tensor, longest: int):
+        self.block_table, self.lens, self.longest = block_table, lens, int(longest)
+
+
+def attention_cross(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor, ctx, source: Source, H: int, K: int, d: int, scale: float,
+                    spans: Optional[torch.Tensor] = None) -> None:
+    """Attention of the step's tokens to their requests' sources, another length than their own and not causal: ``out[t, h] = sum_j p_j v[j]`` with
+    ``p = softmax_j(scale * q[t, h] . k[j])`` over the source's positions, or with ``spans`` (int32 ``[T, 2]``) over those from ``spans[t, 0]`` up to but not
+    including ``spans[t, 1]``; a token that sees nothing gets zeros.  Keys and values lie in pages ``[page, K, page_size, d]`` (a power of two of positions).  Of ``ctx`` it
+    takes ``num_requests``, ``num_decode`` (the first requests, one token each), ``max_query_len`` and ``cu_tokens``; rows of ``q`` ``[T, H * d]`` past the last request's
+    are not read and those of ``out`` stay as they were.  ``q`` may be columns of wider rows."""
+    table, lens = source.block_table, source.lens
+    _on_current_device(q, k_cache, v_cache, out, table, lens, ctx.cu_tokens, spans)
+    T, R, nd = q.shape[0], ctx.num_requests, ctx.num_decode
+    if H <= 0 or K <= 0 or H % K or q.dim() != 2 or q.shape[1] != H * d or (q.shape[1] > 1 and q.stride(1) != 1) or out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise KernelError(f"attention_cross: queries and results are [T, {H * d}] of one dtype ({H} heads over {K} of {d}), got {tuple(q.shape)} and {tuple(out.shape)}")
+    if (k_cache.dtype != q.dtype or v_cache.dtype != q.dtype or k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1] != K or k_cache.shape[3] != d
+            or not k_cache.is_contiguous() or not v_cache.is_contiguous()):
+        raise KernelError(f"attention_cross: caches are contiguous {q.dtype} [pages, {K}, page_size, {d}]")
+    page_size = k_cache.shape[2]
+    if page_size < 1 or page_size & (page_size - 1) or d > 256:
+        raise KernelError(f"attention_cross: pages of a power of two of positions and heads of up to 256, got {page_size} and {d}")
+    _int32("attention_cross", table, lens, ctx.cu_tokens)
+    if table.dim() != 2 or table.shape[0] < R or lens.numel() < R or ctx.cu_tokens.numel() < R + 1 or not 0 <= nd <= R:
+        raise KernelError(f"attention_cross: block_table [{R}, pages], lens [{R}] and cu_tokens [{R + 1}] are wanted")
+    if spans is not None:
+        _int32("attention_cross", spans)
+        if tuple(spans.shape) != (T, 2):
+            raise KernelError(f"attention_cross: spans are [{T}, 2]")
+    if T == 0 or R == 0:
+        return
+    longest = max(0, int(source.longest))
+    for first, n, most, which in ((0, nd, 1, "decode"), (nd, R - nd, ctx.max_query_len, "portions")):
+        if n <= 0:
+            continue
+        if launch_log is not None:
+            rows, size = (n if which == "decode" else T - nd), q.element_size()
+            _cost(size * (2 * rows * H * d + 2 * n * longest * K * d), 4.0 * rows * longest * H * d)
+        _check(_lib("mb_attention_cross").mb_attention_cross(
+            _ptr(q), ctypes.c_longlong(q.stride(0)), _ptr(k_cache), _ptr(v_cache), _ptr(out), _code(q), _ptr(table), _c_int(table.shape[1]), _ptr(lens), _ptr(ctx.cu_tokens),
+            _ptr(spans), _c_int(first), _c_int(n), _c_int(most), _c_int(longest), _c_int(H), _c_int(K), _c_int(d), _c_int(page_size), _c_float(scale), _stream()),
+            f"attention_cross ({which})")
