@@ -1,0 +1,544 @@
+// Attention to an encoder's states on the 5th-generation tensor cores (tcgen05 / TMEM), bfloat16, portions of any length; the formula and the layout
+// of rows are in cross_common.cuh.  Compiled per head size (-DHEAD_DIM, a multiple of 16 up to 128); any number of query heads a kv head up to 128.
+//
+// No mask depends on the order of tokens, so a tile's 128 rows are (token, query head of the group) pairs: 128 / G tokens of all heads that share a kv
+// head, one TMA box of [tokens][G][64 columns]; a portion of seven tokens fills as much of a tile as it can, and keys are fetched once for all of them.
+// A block takes two such tiles (A, B) over the same keys, in blocks of 128:
+//   S = Q K^T     tcgen05.mma 128 x 128 x d, operands in shared memory (TMA, 128-byte swizzle, K-major), S in 128 columns of tensor memory;
+//   P = 2^(S - m) a thread a row: 128 scores in one tcgen05.ld, maximum, exponentials in pairs, P as bfloat16 over the row's own scores (tcgen05.st).  The
+//                 maximum that O and the sum are scaled by follows the true one only when that has moved by more than 8 (2^8, harmless in float32);
+//   O += P V      tcgen05.mma with P from tensor memory, V as it lies in the cache ([key][d], an MN-major operand), O in d columns.
+// While the rows of A work, the tensor core has B's products and the other way round: P V of A and the next S of A, then the same for B.
+// Warps 0..3 are A's rows, 4..7 B's, 8 loads Q and K, 9 loads V, 10 issues the products.  Sums, maxima and O are float32; P is rounded to
+// bfloat16 as the products' operand (its error, 2^-9 of a weight, is that of the rounding of the result; the sum takes the weights before it).
+//
+// Few rows: the blocks of keys are cut over a cluster of up to eight blocks, which add their partial O in shared memory in rank order.
+// What is not there: keys past the source are masked; values past it are zeros (0 * NaN is NaN): whole pages by copies outside the tensor, the page that
+// ends inside by plain stores.  Waits are bounded and record a code in *error_flag.
+#define MB_LIB "attention_cross_tc"
+#define MB_LIB_ID 43
+#include "tc_common.cuh"
+#include "cross_common.cuh"
+
+#ifndef HEAD_DIM
+#error "compile with -DHEAD_DIM=<multiple of 16, at most 128>"
+#endif
+static_assert(HEAD_DIM % 16 == 0 && HEAD_DIM >= 16 && HEAD_DIM <= 128, "heads in steps of 16 up to 128");
+
+#define D HEAD_DIM
+#define NH ((D + 63) / 64)                       // 64-column panels of a row (copies zero-fill past the row's end)
+#define XT_BM 128
+#define XT_BN 128
+#define XT_TILE (NH * 128 * 128)                 // bytes of 128 rows: queries, keys or values
+#define XT_STAGES (NH == 2 ? 2 : 4)              // blocks of keys, and of values, on their way
+#define XT_OLD (D + 4)                           // floats between rows of O for the cluster
+#define XT_BARS 512
+#define XT_SMEM (2 * XT_TILE + 2 * XT_STAGES * XT_TILE + XT_BARS)
+static_assert(2 * XT_BM * XT_OLD * 4 <= 2 * XT_TILE + 2 * XT_STAGES * XT_TILE, "partial results fit the tiles' memory");
+static_assert(XT_SMEM <= 232448 - 4608, "static shared memory is beside it");
+#define XT_TMEM 512                              // S of A, S of B, O of A, O of B: 128 columns each
+#define XT_THREADS 384
+#define XT_MAX_CLUSTER 8
+
+struct CrossTc {
+    CrossArgs a;
+    int* error_flag;
+    int first_request, max_pairs, cache_rows;
+};
+
+__device__ __forceinline__ float xt_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ void of_pair(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// 32 columns of this thread's lane; nothing of v may be used before tmem_ld_wait.
+__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, float* v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
+          "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]),
+          "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]),
+          "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "r"(taddr)
+        : "memory");
+}
+// (the values go through it: the compiler must not use a register of the load ahead of the wait)
+__device__ __forceinline__ void tmem_ld_wait(float* v) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]),
+                   "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]),
+                   "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st32_bits(uint32_t taddr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+          "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]),
+          "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]),
+          "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
+          "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
+        : "memory");
+}
+
+// Waits for a phase; gives up at once if another thread of the block already gave up (`*abort`), and says so itself when its own time limit passes.
+__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort, int* error_flag, int code) {
+    const uint32_t addr = smem_u32(bar);
+    const long long start = clock64();
+    unsigned polls = 0;
+    for (;;) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(addr), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if ((++polls & 31) == 0) {
+            if (*abort) return false;
+            if (clock64() - start > TC_WAIT_LIMIT) { *abort = 1; atomicExch(error_flag, code); return false; }
+        }
+    }
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* error_flag, int code) {
+    return __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort, error_flag, code));
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory"); }
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
+// The MMA with its A operand in tensor memory (row m in lane m, two bf16 per 32-bit column) and B in shared memory.
+__device__ __forceinline__ void umma_bf16_tmem_a(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate, uint32_t elected) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(elected)
+        : "memory");
+}
+
+__global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                                                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CrossTc arg) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t* sQ = smem;                                             // [tile][panel][128 rows][128 B]
+    uint8_t* sK = sQ + 2 * XT_TILE;                                 // [stage][panel][128 rows][128 B]
+    uint8_t* sV = sK + XT_STAGES * XT_TILE;
+    uint64_t* bars = (uint64_t*)(sV + XT_STAGES * XT_TILE);
+    uint64_t* q_full = bars;
+    uint64_t* s_full = bars + 1;                                    // [tile] scores are there (and every product issued before them is done)
+    uint64_t* p_full = bars + 3;                                    // [tile] weights are there (four warps arrive)
+    uint64_t* o_done = bars + 5;                                    // [tile] the last P V is done
+    uint64_t* drained = bars + 7;
+    uint64_t* k_full = bars + 8;                                    // [stage]
+    uint64_t* k_free = k_full + XT_STAGES;
+    uint64_t* v_full = k_free + XT_STAGES;
+    uint64_t* v_free = v_full + XT_STAGES;
+    uint32_t* tmem_slot = (uint32_t*)(v_free + XT_STAGES);
+    volatile int* abort = (volatile int*)(tmem_slot + 1);
+    __shared__ float s_m[2 * XT_BM], s_l[2 * XT_BM];
+    __shared__ int2 s_range[2 * XT_BM];
+    __shared__ int s_first, s_last;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    PDL_ENTER_EARLY();
+    CrossArgs a = arg.a;
+    a.q = pdl_fresh((const char*)a.q); a.v_cache = pdl_fresh((const char*)a.v_cache); a.k_cache = pdl_fresh((const char*)a.k_cache);
+    a.block_table = pdl_fresh(a.block_table); a.lens = pdl_fresh(a.lens); a.cu_tokens = pdl_fresh(a.cu_tokens); a.spans = pdl_fresh(a.spans);
+    int* error_flag = arg.error_flag;
+    const int r = arg.first_request + blockIdx.x / arg.max_pairs, pair = blockIdx.x % arg.max_pairs, kh = blockIdx.y;
+    const int rank = blockIdx.z, cluster = gridDim.z, G = a.G, per_tile = XT_BM / G;
+    const int tok0 = a.cu_tokens[r] + pair * 2 * per_tile, left = a.cu_tokens[r + 1] - tok0;
+    if (left <= 0) return;                                          // (all blocks of a cluster)
+    if ((smem_u32(smem) & 1023u) != 0) { if (tid == 0) atomicExch(error_flag, 40); return; }
+    const bool two = left > per_tile;                               // tile B has rows
+    const int len = max(0, min(a.lens[r], a.max_pages << a.page_shift));
+    const int* table = a.block_table + (size_t)r * a.max_pages;
+    if (tid == 0) {
+        mbar_init(q_full, 1); mbar_init(drained, 1);
+        for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1); }
+        for (int i = 0; i < XT_STAGES; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_free[i], 1); mbar_init(&v_full[i], 1); mbar_init(&v_free[i], 1); }
+        *abort = 0;
+        s_first = len; s_last = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) { __syncwarp(); tmem_alloc<false>(tmem_slot, XT_TMEM); }
+    __syncthreads();
+    // this thread's row (threads 0..255): tile, token, head
+    const int tile = warp >> 2, in_tile = tid & (XT_BM - 1), my_tok = tile * per_tile + in_tile / G, my_head = kh * G + in_tile % G;
+    const bool mine = tid < 2 * XT_BM && in_tile < per_tile * G && my_tok < left;
+    int2 range = make_int2(0, 0);
+    if (mine) range = cross_range(a, tok0 + my_tok, len);
+    if (tid < 2 * XT_BM) {
+        s_range[tid] = range;
+        if (a.spans == nullptr) { if (tid == 0) { s_first = 0; s_last = len; } }
+        else if (range.y > range.x) { atomicMin(&s_first, range.x); atomicMax(&s_last, range.y); }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_base = *tmem_slot;
+    const int first_block = s_first / XT_BN, blocks_all = s_last > s_first ? (s_last + XT_BN - 1) / XT_BN - first_block : 0;
+    const int share = (blocks_all + cluster - 1) / cluster;
+    const int block0 = first_block + rank * share, nblk = max(0, min(share, blocks_all - rank * share));
+    float m_used = -INFINITY, l_run = 0.0f;
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == 8 || warp == 9) {
+            // ---- the loaders: a lane a box (a page's rows of one panel), as soon as the block's buffer is free; where the boxes lie is looked up a block ahead ----
+            const bool keys = warp == 8;
+            const CUtensorMap* map = keys ? &map_k : &map_v;
+            uint64_t* full = keys ? k_full : v_full;
+            uint64_t* freed = keys ? k_free : v_free;
+            const int page = 1 << a.page_shift, boxes = XT_BN >> a.page_shift, box = lane % boxes, panel = lane / boxes;
+            const bool loads = panel < NH;
+            auto row_of = [&](int i) -> int {                       // the box's first row among the cache's rows (past them: zeros)
+                const int key = (block0 + i) * XT_BN + box * page;
+                if (!loads || i >= nblk || key >= len) return arg.cache_rows;
+                return (int)(((unsigned)table[key >> a.page_shift] * (unsigned)a.K + (unsigned)kh) << a.page_shift);
+            };
+            if (keys && nblk > 0 && lane < NH * (two ? 2 : 1)) {
+                const int t = lane / NH, p = lane % NH;
+                if (lane == 0) mbar_expect_tx(q_full, (uint32_t)((two ? 2 : 1) * NH * per_tile * G * 128));
+                __syncwarp(__activemask());
+                tma_load_3d(sQ + t * XT_TILE + p * (XT_BM * 128), &map_q, p * 64, kh * G, tok0 + t * per_tile, q_full);
+            }
+            __syncwarp();
+            int row = row_of(0);
+            bool ok = true;
+            int asked = 0;
+            for (int i = 0; ok && i < nblk; ++i) {
+                const int st = i % XT_STAGES;
+                if (i >= XT_STAGES) ok = warp_wait(&freed[st], ((i / XT_STAGES) - 1) & 1, abort, error_flag, 41);
+                if (!ok) break;
+                uint8_t* dst = (keys ? sK : sV) + st * XT_TILE;
+                // the page that the source ends in: its values by plain stores, zeros from there on
+                const int tail = keys ? 0 : len - (block0 + i) * XT_BN, cut = tail > 0 && tail < XT_BN ? tail >> a.page_shift : XT_BN;
+                const bool partial = cut < XT_BN && (tail & (page - 1)) != 0;
+                if (partial) {
+                    const bf16* src = cross_row<bf16>(a, a.v_cache, table, kh, (block0 + i) * XT_BN + cut * page);
+                    for (int x = lane; x < page * NH * 8; x += 32) {
+                        const int rw = x / (NH * 8), c = x % (NH * 8), at = cut * page + rw;
+                        uint4 v = make_uint4(0, 0, 0, 0);
+                        if (at < tail && c * 8 < D) v = *reinterpret_cast<const uint4*>(src + (size_t)rw * D + c * 8);
+                        *reinterpret_cast<uint4*>(dst + (c >> 3) * (XT_BN * 128) + at * 128 + (((c & 7) ^ (at & 7)) << 4)) = v;
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
+                if (lane == 0) mbar_expect_tx(&full[st], (uint32_t)(XT_TILE - (partial ? NH * page * 128 : 0)));
+                __syncwarp();
+                if (loads && !(partial && box == cut)) tma_load_2d(dst + panel * (XT_BN * 128) + box * page * 128, map, panel * 64, row, &full[st]);
+                row = row_of(i + 1);
+                asked = i + 1;
+            }
+            // (what was asked for has to land before the block ends; where all went well the issuer has waited for it)
+            if (!ok)
+                for (int i = max(0, asked - XT_STAGES); i < asked; ++i) mbar_wait_warp(&full[i % XT_STAGES], (i / XT_STAGES) & 1);
+        } else if (warp == 10) {
+            // ---- the issuer ----
+            constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(XT_BN >> 3) << 17) | ((uint32_t)(XT_BM >> 4) << 24);
+            constexpr uint32_t idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(XT_BM >> 4) << 24);
+            const uint32_t elected = elect_one(), tmem = warp_same(tmem_base);
+            const int blocks = warp_same(nblk);
+            const int tiles = warp_same(two ? 2 : 1);
+            auto scores = [&](int t, int i) {
+                const uint64_t qdesc = umma_desc(smem_u32(sQ + t * XT_TILE)), kdesc = umma_desc(smem_u32(sK + (i % XT_STAGES) * XT_TILE));
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    const uint32_t step = (uint32_t)((kk / 4) * (128 * 128 >> 4) + 2 * (kk % 4));
+                    umma_bf16(tmem + (uint32_t)(t * XT_BN), qdesc + step, kdesc + step, idesc_s, kk > 0 ? 1u : 0u, elected);
+                }
+                umma_commit(&s_full[t], elected);
+            };
+            auto values = [&](int t, int i) {
+                const uint64_t vdesc = umma_desc_mn(smem_u32(sV + (i % XT_STAGES) * XT_TILE), XT_BN * 128);
+#pragma unroll
+                for (int kk = 0; kk < XT_BN / 16; ++kk)
+                    umma_bf16_tmem_a(tmem + (uint32_t)(2 * XT_BN + t * 128), tmem + (uint32_t)(t * XT_BN + kk * 8), vdesc + (uint32_t)(kk * (2048 >> 4)), idesc_pv,
+                                     (i > 0 || kk > 0) ? 1u : 0u, elected);
+            };
+            bool ok = blocks > 0 && warp_wait(q_full, 0, abort, error_flag, 42) && warp_wait(&k_full[0], 0, abort, error_flag, 42);
+            if (ok) {
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                for (int t = 0; t < tiles; ++t) scores(t, 0);
+                umma_commit(&k_free[0], elected);
+            }
+            for (int i = 0; ok && i < blocks; ++i) {
+                const int st = i % XT_STAGES, nx = (i + 1) % XT_STAGES;
+                ok = warp_wait(&v_full[st], (i / XT_STAGES) & 1, abort, error_flag, 43);
+                for (int t = 0; ok && t < tiles; ++t) {
+                    ok = warp_wait(&p_full[t], i & 1, abort, error_flag, 44);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    values(t, i);
+                    if (t == tiles - 1) umma_commit(&v_free[st], elected);
+                    if (i + 1 < blocks) {
+                        // (S goes where P lies: the tensor core takes the products in the order they were issued)
+                        if (t == 0) ok = warp_wait(&k_full[nx], ((i + 1) / XT_STAGES) & 1, abort, error_flag, 45);
+                        if (!ok) break;
+                        scores(t, i + 1);
+                        if (t == tiles - 1) umma_commit(&k_free[nx], elected);
+                    } else {
+                        umma_commit(&o_done[t], elected);
+                    }
+                }
+            }
+            if (!ok && blocks > 0) {                                // (and what was issued has to end)
+                umma_commit(drained, elected);
+                mbar_wait_warp(drained, 0);
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        // ---- the rows ----
+        const uint32_t lane_base = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t s_col = lane_base + (uint32_t)(tile * XT_BN), o_col = lane_base + (uint32_t)(2 * XT_BN + tile * 128);
+        const float sl2 = a.scale * 1.4426950408889634f;
+        bool ok = true;
+        const int steps = tile == 0 || two ? nblk : 0;
+        for (int i = 0; i < steps; ++i) {
+            ok = warp_wait(&s_full[tile], i & 1, abort, error_flag, 46);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            float s[XT_BN];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld32_async(s_col + c * 32, s + c * 32);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld_wait(s + c * 32);
+            const int key0 = (block0 + i) * XT_BN, from = range.x - key0, to = range.y - key0;
+            if (__any_sync(0xffffffffu, from > 0 || to < XT_BN)) {
+#pragma unroll
+                for (int j = 0; j < XT_BN; ++j)
+                    if (j < from || j >= to) s[j] = -INFINITY;
+            }
+            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int j = 0; j < XT_BN; j += 8)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) m4[e] = max3(m4[e], s[j + 2 * e], s[j + 2 * e + 1]);
+            const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+            const float m_true = fmaxf(m_used, mx * sl2);
+            const bool raise = m_true > m_used + 8.0f || (m_used == -INFINITY && m_true != -INFINITY);
+            const float m_new = raise ? m_true : m_used;
+            const float corr = raise ? xt_exp2(m_used - m_new) : 1.0f;
+            if (i > 0 && __any_sync(0xffffffffu, raise)) {          // (P V of the blocks ahead is done: these scores were issued after it)
+#pragma unroll
+                for (int c = 0; c < D / 16; ++c) {
+                    float o[16];
+                    tmem_ld16(o_col + c * 16, o);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) o[j] *= corr;
+                    tmem_st16(o_col + c * 16, o);
+                }
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            }
+            m_used = m_new;
+            const float base = m_used == -INFINITY ? 0.0f : m_used;
+            const uint64_t scale2 = pair_of(sl2, sl2), base2 = pair_of(-base, -base);
+            uint64_t sum2[2] = {0, 0};
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t packed[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    const uint64_t x = fma_pair(pair_of(s[c * 64 + 2 * j], s[c * 64 + 2 * j + 1]), scale2, base2);
+                    float x0, x1;
+                    of_pair(x, x0, x1);
+                    const float p0 = xt_exp2(x0), p1 = xt_exp2(x1);
+                    sum2[j & 1] = add_pair(sum2[j & 1], pair_of(p0, p1));
+                    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(packed[j]) : "f"(p1), "f"(p0));
+                }
+                tmem_st32_bits(s_col + c * 32, packed);
+            }
+            float u0, u1;
+            of_pair(add_pair(sum2[0], sum2[1]), u0, u1);
+            l_run = l_run * corr + (u0 + u1);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[tile]);
+        }
+        if (ok && steps > 0) ok = warp_wait(&o_done[tile], 0, abort, error_flag, 47);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (cluster == 1) {
+            bf16* dst = (bf16*)a.out + ((size_t)(tok0 + my_tok) * a.K * G + my_head) * D;
+            const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
+            bool odd = false;
+            if (ok && (tile == 0 || two)) {
+#pragma unroll
+                for (int c = 0; c < D / 16; ++c) {
+                    float o[16];
+                    if (steps > 0) tmem_ld16(o_col + c * 16, o);
+                    if (mine) {
+                        uint32_t w[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float x = range.y > range.x ? o[2 * j] * inv : 0.0f, y = range.y > range.x ? o[2 * j + 1] * inv : 0.0f;
+                            odd |= !(fabsf(x) <= 3.0e38f) || !(fabsf(y) <= 3.0e38f);
+                            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[j]) : "f"(y), "f"(x));
+                        }
+                        reinterpret_cast<uint4*>(dst)[c * 2] = make_uint4(w[0], w[1], w[2], w[3]);
+                        reinterpret_cast<uint4*>(dst)[c * 2 + 1] = make_uint4(w[4], w[5], w[6], w[7]);
+                    }
+                }
+                if (a.spans != nullptr) {
+                    unsigned which = __ballot_sync(0xffffffffu, odd);
+                    while (which != 0) {
+                        const int src = __ffs(which) - 1;
+                        which &= which - 1;
+                        const int tok = __shfl_sync(0xffffffffu, my_tok, src), head = __shfl_sync(0xffffffffu, my_head, src);
+                        const int2 rg = make_int2(__shfl_sync(0xffffffffu, range.x, src), __shfl_sync(0xffffffffu, range.y, src));
+                        __syncwarp();
+                        cross_row_alone<bf16>(a, tok0 + tok, head, r, rg);
+                    }
+                }
+            }
+        } else {
+            // partial results into the tiles' memory, once every product of both tiles is done
+            if (ok && two && nblk > 0) ok = warp_wait(&o_done[1 - tile], 0, abort, error_flag, 47);
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            float* sO = (float*)smem + (size_t)tid * XT_OLD;
+            s_m[tid] = m_used; s_l[tid] = l_run;
+            if (ok && (tile == 0 || two)) {
+#pragma unroll
+                for (int c = 0; c < D / 16; ++c) {
+                    float o[16];
+                    if (steps > 0) tmem_ld16(o_col + c * 16, o);
+                    else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) o[j] = 0.0f;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(sO + c * 16 + 4 * j) = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                }
+            }
+        }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 0) { __syncwarp(); tmem_free<false>(tmem_base, XT_TMEM); }
+    if (cluster > 1) {
+        cross_cluster_sync();
+        // block `rank` finishes rows rank, rank + cluster, ...: a warp a row, the partial results in rank order
+        const float* sO = (const float*)smem;
+        for (int row = rank + warp * cluster; row < 2 * XT_BM; row += (XT_THREADS / 32) * cluster) {
+            const int in = row & (XT_BM - 1), tok = (row / XT_BM) * per_tile + in / G, head = kh * G + in % G;
+            if (in >= per_tile * G || tok >= left) continue;
+            float w[XT_MAX_CLUSTER], top = -INFINITY, sum = 0.0f;
+#pragma unroll
+            for (int c = 0; c < XT_MAX_CLUSTER; ++c) {
+                w[c] = c < cluster ? cross_peer(smem_u32(&s_m[row]), c) : -INFINITY;
+                top = fmaxf(top, w[c]);
+            }
+            const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+            for (int c = 0; c < XT_MAX_CLUSTER; ++c)
+                if (c < cluster) { w[c] = xt_exp2(w[c] - base); sum += w[c] * cross_peer(smem_u32(&s_l[row]), c); }
+            const int2 rg = s_range[row];
+            bf16* dst = (bf16*)a.out + ((size_t)(tok0 + tok) * a.K * G + head) * D;
+            bool odd = false;
+            for (int x = lane; x < D; x += 32) {
+                float v = 0.0f;
+#pragma unroll
+                for (int c = 0; c < XT_MAX_CLUSTER; ++c)
+                    if (c < cluster) v = fmaf(w[c], cross_peer(smem_u32(sO + (size_t)row * XT_OLD + x), c), v);
+                v = rg.y > rg.x && sum != 0.0f ? v / sum : 0.0f;
+                odd |= !(fabsf(v) <= 3.0e38f);
+                dst[x] = __float2bfloat16_rn(v);
+            }
+            if (a.spans != nullptr && __any_sync(0xffffffffu, odd)) { __syncwarp(); cross_row_alone<bf16>(a, tok0 + tok, head, r, rg); }
+        }
+        cross_cluster_sync();                                       // (a block's shared memory is read until here)
+    }
+}
+
+// ---- host side ----
+static int map_rows(CUtensorMap* map, const void* base, uint64_t rows, uint32_t box_rows) {
+    EncodeTiled enc = encode_tiled();
+    if (enc == nullptr) return MB_ERR_BAD_SIZE;
+    cuuint64_t dims[2] = {D, rows};
+    cuuint64_t strides[1] = {D * 2};
+    cuuint32_t box[2] = {64, box_rows};
+    cuuint32_t elem[2] = {1, 1};
+    const CUresult rc = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return rc == CUDA_SUCCESS ? 0 : 1000 + (int)rc;
+}
+static int map_queries(CUtensorMap* map, const void* q, long long stride, int H, int tokens, int G, int per_tile) {
+    EncodeTiled enc = encode_tiled();
+    if (enc == nullptr) return MB_ERR_BAD_SIZE;
+    cuuint64_t dims[3] = {D, (cuuint64_t)H, (cuuint64_t)tokens};
+    cuuint64_t strides[2] = {D * 2, (cuuint64_t)stride * 2};
+    cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)per_tile};
+    cuuint32_t elem[3] = {1, 1, 1};
+    const CUresult rc = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return rc == CUDA_SUCCESS ? 0 : 1000 + (int)rc;
+}
+
+// Requests first_request .. first_request + requests - 1 (none with more than max_query tokens) of a step of `tokens` tokens.  chunks: 1, 2, 4 or 8 blocks
+// share a tile pair's keys.  Pages of 16 to 128 positions; q, caches and out at 16 bytes, q_stride in whole 16-byte steps.
+MB_API int mb_attention_cross_tc(const void* q, long long q_stride, const void* k_cache, const void* v_cache, void* out, const int* block_table, int max_pages,
+                                 const int* lens, const int* cu_tokens, const int* spans, int first_request, int requests, int max_query, int tokens, int chunks, int H,
+                                 int K, int page_size, long long cache_pages, float scale, int* error_flag, cudaStream_t s) {
+    if (requests <= 0 || max_query <= 0) return 0;
+    int shift = -1;
+    for (int b = 4; b < 8; ++b)
+        if ((1 << b) == page_size) shift = b;
+    const long long cache_rows = cache_pages * K * page_size;
+    if (shift < 0 || K <= 0 || H <= 0 || H % K != 0 || H / K > XT_BM || K > 65535 || cache_rows <= 0 || cache_rows > 0x7fffff00LL ||
+        ((long long)max_pages << shift) > 0x7fffff00LL || (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15) != 0 || q_stride % 8 != 0 ||
+        !(chunks == 1 || chunks == 2 || chunks == 4 || chunks == XT_MAX_CLUSTER))
+        return MB_ERR_BAD_SIZE;
+    const int G = H / K, per_tile = XT_BM / G;
+    const long long pairs = (max_query + 2LL * per_tile - 1) / (2 * per_tile);
+    if (pairs * requests > 0x7fffffffLL) return MB_ERR_BAD_SIZE;
+    static LaunchSmem allowed;
+    int rc = allowed.allow(attention_cross_tc_kernel, XT_SMEM);
+    if (rc != 0) return rc;
+    CUtensorMap mq, mk, mv;
+    if ((rc = map_queries(&mq, q, q_stride, H, tokens, G, per_tile)) != 0) return rc;
+    if ((rc = map_rows(&mk, k_cache, (uint64_t)cache_rows, (uint32_t)page_size)) != 0) return rc;
+    if ((rc = map_rows(&mv, v_cache, (uint64_t)cache_rows, (uint32_t)page_size)) != 0) return rc;
+    const CrossTc arg = {{q, k_cache, v_cache, out, block_table, lens, cu_tokens, spans, q_stride, max_pages, K, G, D, shift, scale}, error_flag, first_request, (int)pairs,
+                         (int)cache_rows};
+    return launch_kernel(attention_cross_tc_kernel, dim3((unsigned)(requests * pairs), K, chunks), dim3(XT_THREADS), XT_SMEM, s, chunks, mq, mk, mv, arg);
+}

@@ -2924,6 +2924,24 @@ class Source:
         self.block_table, self.lens, self.longest = block_table, lens, int(longest)
 
 
+def cross_tc_supported(dtype, H: int, K: int, d: int, page_size: int) -> bool:
+    """Whether the tensor-core kernel takes this layout (the others go to the 32-bit one): bfloat16, heads in steps of 16 up to 128, up to 128 query heads a kv
+    head, pages of 16 to 128 positions."""
+    return dtype == torch.bfloat16 and d % 16 == 0 and 16 <= d <= 128 and H // K <= 128 and page_size in (16, 32, 64, 128)
+
+
+def _cross_tc_lib(d: int):
+    return build.load(f"mb_attention_cross_tc_d{d}", ["attention_cross_tc.cu"], [f"HEAD_DIM={d}"])
+
+
+def cross_chunks(blocks: int, longest: int) -> int:
+    """Over how many blocks of a cluster (1, 2, 4 or 8) a tile pair's keys are cut: as many as fill the SMs, none with fewer than 256 keys."""
+    chunks = 1
+    while chunks < 8 and blocks * chunks * 2 <= SM_COUNT and chunks * 256 < longest:
+        chunks *= 2
+    return chunks
+
+
 def attention_cross(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor, ctx, source: Source, H: int, K: int, d: int, scale: float,
                     spans: Optional[torch.Tensor] = None) -> None:
     """Attention of the step's tokens to their requests' sources, another length than their own and not causal: ``out[t, h] = sum_j p_j v[j]`` with
@@ -2949,15 +2967,25 @@ def attention_cross(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         _int32("attention_cross", spans)
         if tuple(spans.shape) != (T, 2):
             raise KernelError(f"attention_cross: spans are [{T}, 2]")
+    if not 0.0 < scale < float("inf"):
+        raise KernelError(f"attention_cross: scale is a positive number, got {scale}")
     if T == 0 or R == 0:
         return
     longest = max(0, int(source.longest))
+    tc = cross_tc_supported(q.dtype, H, K, d, page_size) and q.stride(0) % 8 == 0 and all(x.data_ptr() % 16 == 0 for x in (q, k_cache, v_cache, out)) and k_cache.shape[0] * K * page_size < 0x7fffff00 and k_cache.shape[0] > 0
     for first, n, most, which in ((0, nd, 1, "decode"), (nd, R - nd, ctx.max_query_len, "portions")):
         if n <= 0:
             continue
         if launch_log is not None:
             rows, size = (n if which == "decode" else T - nd), q.element_size()
             _cost(size * (2 * rows * H * d + 2 * n * longest * K * d), 4.0 * rows * longest * H * d)
+        if tc:
+            tiles = -(-most * (H // K) // (2 * (128 // (H // K) * (H // K))))
+            _check(_cross_tc_lib(d).mb_attention_cross_tc(
+                _ptr(q), ctypes.c_longlong(q.stride(0)), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(table), _c_int(table.shape[1]), _ptr(lens), _ptr(ctx.cu_tokens),
+                _ptr(spans), _c_int(first), _c_int(n), _c_int(most), _c_int(T), _c_int(cross_chunks(min(n * tiles, n + (T * (H // K)) // 256) * K, longest)), _c_int(H), _c_int(K), _c_int(page_size),
+                ctypes.c_longlong(k_cache.shape[0]), _c_float(scale), _ptr(_scratch_for(q.device).error), _stream()), f"attention_cross ({which}, tensor cores)")
+            continue
         _check(_lib("mb_attention_cross").mb_attention_cross(
             _ptr(q), ctypes.c_longlong(q.stride(0)), _ptr(k_cache), _ptr(v_cache), _ptr(out), _code(q), _ptr(table), _c_int(table.shape[1]), _ptr(lens), _ptr(ctx.cu_tokens),
             _ptr(spans), _c_int(first), _c_int(n), _c_int(most), _c_int(longest), _c_int(H), _c_int(K), _c_int(d), _c_int(page_size), _c_float(scale), _stream()),
