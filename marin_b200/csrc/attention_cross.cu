@@ -51,7 +51,7 @@ __device__ __forceinline__ void cross_tile(float* dst, const CrossArgs& a, const
 }
 
 template <typename T, int BM, int DCH>
-__global__ void __launch_bounds__(256) attention_cross_kernel(CrossArgs a, int first_request, int max_tiles, int whole) {
+__global__ void __launch_bounds__(256) attention_cross_kernel(const __grid_constant__ CrossArgs arg, int first_request, int max_tiles, int whole) {
     constexpr int RM = BM / 16, LD = DCH * 64 + 4;
     extern __shared__ __align__(16) float cx_smem[];
     float* sQ = cx_smem;                                            // [BM][LD]; later the partial results
@@ -61,6 +61,7 @@ __global__ void __launch_bounds__(256) attention_cross_kernel(CrossArgs a, int f
     __shared__ float s_m[BM], s_l[BM];
     __shared__ int s_lo[BM], s_hi[BM], s_first, s_last;
     PDL_ENTER();
+    CrossArgs a = arg;
     a.q = pdl_fresh((const char*)a.q); a.k_cache = pdl_fresh((const char*)a.k_cache); a.v_cache = pdl_fresh((const char*)a.v_cache);
     a.block_table = pdl_fresh(a.block_table); a.lens = pdl_fresh(a.lens); a.cu_tokens = pdl_fresh(a.cu_tokens); a.spans = pdl_fresh(a.spans);
     const int r = first_request + blockIdx.x / max_tiles, tile = blockIdx.x % max_tiles, kh = blockIdx.y;
@@ -223,7 +224,7 @@ __global__ void __launch_bounds__(256) attention_cross_kernel(CrossArgs a, int f
             odd |= !(fabsf(v) <= 3.0e38f);
             out[c] = from_f32<T>(v);
         }
-        if (a.spans != nullptr && __any_sync(0xffffffffu, odd)) cross_row_alone<T>(a, t, head, r, make_int2(s_lo[row], s_hi[row]));
+        if (a.spans != nullptr && __any_sync(0xffffffffu, odd)) cross_row_alone<T>(arg, t, head, r, make_int2(s_lo[row], s_hi[row]));
     }
     if (gridDim.z > 1) cross_cluster_sync();                        // (a block's shared memory is read until here)
 }

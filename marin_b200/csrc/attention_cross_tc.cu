@@ -5,11 +5,12 @@
 // head, one TMA box of [tokens][G][64 columns]; a portion of seven tokens fills as much of a tile as it can, and keys are fetched once for all of them.
 // A block takes two such tiles (A, B) over the same keys, in blocks of 128:
 //   S = Q K^T     tcgen05.mma 128 x 128 x d, operands in shared memory (TMA, 128-byte swizzle, K-major), S in 128 columns of tensor memory;
-//   P = 2^(S - m) a thread a row: 128 scores in one tcgen05.ld, maximum, exponentials in pairs, P as bfloat16 over the row's own scores (tcgen05.st).  The
+//   P = 2^(S - m) two threads a row: 64 scores each by tcgen05.ld, maximum, exponentials in pairs, P as bfloat16 over the row's own scores (tcgen05.st).  The
 //                 maximum that O and the sum are scaled by follows the true one only when that has moved by more than 8 (2^8, harmless in float32);
 //   O += P V      tcgen05.mma with P from tensor memory, V as it lies in the cache ([key][d], an MN-major operand), O in d columns.
 // While the rows of A work, the tensor core has B's products and the other way round: P V of A and the next S of A, then the same for B.
-// Warps 0..3 are A's rows, 4..7 B's, 8 loads Q and K, 9 loads V, 10 issues the products.  Sums, maxima and O are float32; P is rounded to
+// Warps 0..7 are A's rows, 8..15 B's (two threads a row, 64 keys of a block each: a scheduler has two warps for every tile), 16 loads Q and K, 17 loads V, 18 and 19
+// issue A's and B's products.  Sums, maxima and O are float32; P is rounded to
 // bfloat16 as the products' operand (its error, 2^-9 of a weight, is that of the rounding of the result; the sum takes the weights before it).
 //
 // Few rows: the blocks of keys are cut over a cluster of up to eight blocks, which add their partial O in shared memory in rank order.
@@ -28,17 +29,22 @@ static_assert(HEAD_DIM % 16 == 0 && HEAD_DIM >= 16 && HEAD_DIM <= 128, "heads in
 #define D HEAD_DIM
 #define NH ((D + 63) / 64)                       // 64-column panels of a row (copies zero-fill past the row's end)
 #define XT_BM 128
-#define XT_BN 128
-#define XT_TILE (NH * 128 * 128)                 // bytes of 128 rows: queries, keys or values
-#define XT_STAGES (NH == 2 ? 2 : 4)              // blocks of keys, and of values, on their way
+#define XT_BN 64                                 // keys of a block
+#define XT_TILE (NH * XT_BM * 128)               // bytes of a tile of queries
+#define XT_KV (NH * XT_BN * 128)                 // bytes of a block of keys, or of values
+#define XT_STAGES 4                             // blocks of keys, and of values, on their way
 #define XT_OLD (D + 4)                           // floats between rows of O for the cluster
 #define XT_BARS 512
-#define XT_SMEM (2 * XT_TILE + 2 * XT_STAGES * XT_TILE + XT_BARS)
-static_assert(2 * XT_BM * XT_OLD * 4 <= 2 * XT_TILE + 2 * XT_STAGES * XT_TILE, "partial results fit the tiles' memory");
+#define XT_SMEM (2 * XT_TILE + 2 * XT_STAGES * XT_KV + XT_BARS)
+static_assert(2 * XT_BM * XT_OLD * 4 <= 2 * XT_TILE + 2 * XT_STAGES * XT_KV, "partial results fit the tiles' memory");
 static_assert(XT_SMEM <= 232448 - 4608, "static shared memory is beside it");
-#define XT_TMEM 512                              // S of A, S of B, O of A, O of B: 128 columns each
+#define XT_TMEM 512                              // two S buffers of A, of B (64 columns each), O of A, O of B (128)
+#define XT_O_COL 256
 #define XT_THREADS 384
 #define XT_MAX_CLUSTER 8
+#ifndef XT_POLY
+#define XT_POLY 0                                // of eight pairs of scores, how many go by the polynomial
+#endif
 
 struct CrossTc {
     CrossArgs a;
@@ -67,6 +73,30 @@ __device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c)
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
     return d;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+// 2^x of a pair without the special-function unit, for x in [-126, 126] (below: 2^-126): x = n + f with n the nearest whole number (1.5 * 2^23 added and taken
+// off again), 2^f by a cubic fitted on [-1/2, 1/2] for the least largest relative error, 7.5e-5 (a weight is rounded to bfloat16, 2e-3, next), n added to the exponent.
+__device__ __forceinline__ void exp2_pair_poly(uint64_t x, float& p0, float& p1) {
+    float x0, x1, n0, n1;
+    of_pair(x, x0, x1);
+    x = pair_of(max_nan(x0, -126.0f), max_nan(x1, -126.0f));
+    uint64_t magic, t, n, f, p;
+    magic = pair_of(12582912.0f, 12582912.0f);
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(t) : "l"(x), "l"(magic));
+    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(n) : "l"(t), "l"(magic));
+    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(f) : "l"(x), "l"(n));
+    p = fma_pair(pair_of(0.05517167f, 0.05517167f), f, pair_of(0.24261113f, 0.24261113f));
+    p = fma_pair(p, f, pair_of(0.69326097f, 0.69326097f));
+    p = fma_pair(p, f, pair_of(0.99992806f, 0.99992806f));
+    of_pair(p, p0, p1);
+    of_pair(t, n0, n1);
+    p0 = __int_as_float(__float_as_int(p0) + (__float_as_int(n0) << 23));
+    p1 = __int_as_float(__float_as_int(p1) + (__float_as_int(n1) << 23));
+}
 __device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
@@ -94,14 +124,11 @@ __device__ __forceinline__ void tmem_ld_wait(float* v) {
                  :
                  : "memory");
 }
-__device__ __forceinline__ void tmem_st32_bits(uint32_t taddr, const uint32_t* v) {
+__device__ __forceinline__ void tmem_st16_bits(uint32_t taddr, const uint32_t* v) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
         ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-          "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]),
-          "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]),
-          "r"(v[30]), "r"(v[31])
+          "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* v) {
@@ -112,22 +139,25 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* v) {
         : "memory");
 }
 
+__device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
 // Waits for a phase; gives up at once if another thread of the block already gave up (`*abort`), and says so itself when its own time limit passes.
+// (The clock is asked only where the phase was not there at once: reading it cost as much as the wait.)
 __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort, int* error_flag, int code) {
-    const uint32_t addr = smem_u32(bar);
+    if (mbar_try(bar, parity)) return true;
     const long long start = clock64();
-    unsigned polls = 0;
-    for (;;) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done)
-            : "r"(addr), "r"(parity)
-            : "memory");
-        if (done) return true;
-        if ((++polls & 31) == 0) {
+    for (unsigned polls = 1;; ++polls) {
+        if (mbar_try(bar, parity)) return true;
+        if ((polls & 31) == 0) {
             if (*abort) return false;
             if (clock64() - start > TC_WAIT_LIMIT) { *abort = 1; atomicExch(error_flag, code); return false; }
         }
@@ -159,14 +189,14 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* sQ = smem;                                             // [tile][panel][128 rows][128 B]
     uint8_t* sK = sQ + 2 * XT_TILE;                                 // [stage][panel][128 rows][128 B]
-    uint8_t* sV = sK + XT_STAGES * XT_TILE;
-    uint64_t* bars = (uint64_t*)(sV + XT_STAGES * XT_TILE);
+    uint8_t* sV = sK + XT_STAGES * XT_KV;
+    uint64_t* bars = (uint64_t*)(sV + XT_STAGES * XT_KV);
     uint64_t* q_full = bars;
-    uint64_t* s_full = bars + 1;                                    // [tile] scores are there (and every product issued before them is done)
-    uint64_t* p_full = bars + 3;                                    // [tile] weights are there (four warps arrive)
-    uint64_t* o_done = bars + 5;                                    // [tile] the last P V is done
-    uint64_t* drained = bars + 7;
-    uint64_t* k_full = bars + 8;                                    // [stage]
+    uint64_t* s_full = bars + 1;                                    // [tile][buffer] scores are there
+    uint64_t* p_full = bars + 5;                                    // [tile][buffer] weights are there (four warps arrive)
+    uint64_t* o_done = bars + 9;                                    // [tile][buffer] P V of the buffer's weights is done
+    uint64_t* drained = bars + 13;
+    uint64_t* k_full = bars + 15;                                   // [stage]
     uint64_t* k_free = k_full + XT_STAGES;
     uint64_t* v_full = k_free + XT_STAGES;
     uint64_t* v_free = v_full + XT_STAGES;
@@ -186,13 +216,14 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
     const int tok0 = a.cu_tokens[r] + pair * 2 * per_tile, left = a.cu_tokens[r + 1] - tok0;
     if (left <= 0) return;                                          // (all blocks of a cluster)
     if ((smem_u32(smem) & 1023u) != 0) { if (tid == 0) atomicExch(error_flag, 40); return; }
-    const bool two = left > per_tile;                               // tile B has rows
+    // Where the rows fit one tile, both halves of the block work on it: B has the same rows and the blocks of odd number, A those of even number.
+    const bool two = left > per_tile;
     const int len = max(0, min(a.lens[r], a.max_pages << a.page_shift));
     const int* table = a.block_table + (size_t)r * a.max_pages;
     if (tid == 0) {
-        mbar_init(q_full, 1); mbar_init(drained, 1);
-        for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1); }
-        for (int i = 0; i < XT_STAGES; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_free[i], 1); mbar_init(&v_full[i], 1); mbar_init(&v_free[i], 1); }
+        mbar_init(q_full, 1); mbar_init(&drained[0], 1); mbar_init(&drained[1], 1);
+        for (int i = 0; i < 4; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1); }
+        for (int i = 0; i < XT_STAGES; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_free[i], two ? 2 : 1); mbar_init(&v_full[i], 1); mbar_init(&v_free[i], two ? 2 : 1); }
         *abort = 0;
         s_first = len; s_last = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -200,11 +231,11 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
     if (warp == 0) { __syncwarp(); tmem_alloc<false>(tmem_slot, XT_TMEM); }
     __syncthreads();
     // this thread's row (threads 0..255): tile, token, head
-    const int tile = warp >> 2, in_tile = tid & (XT_BM - 1), my_tok = tile * per_tile + in_tile / G, my_head = kh * G + in_tile % G;
-    const bool mine = tid < 2 * XT_BM && in_tile < per_tile * G && my_tok < left;
+    const int tile = warp >> 2, in_tile = tid & (XT_BM - 1), my_tok = (two ? tile * per_tile : 0) + in_tile / G, my_head = kh * G + in_tile % G;
+    const bool mine = warp < 8 && in_tile < per_tile * G && my_tok < left;
     int2 range = make_int2(0, 0);
     if (mine) range = cross_range(a, tok0 + my_tok, len);
-    if (tid < 2 * XT_BM) {
+    if (warp < 8) {
         s_range[tid] = range;
         if (a.spans == nullptr) { if (tid == 0) { s_first = 0; s_last = len; } }
         else if (range.y > range.x) { atomicMin(&s_first, range.x); atomicMax(&s_last, range.y); }
@@ -216,22 +247,21 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
     const int first_block = s_first / XT_BN, blocks_all = s_last > s_first ? (s_last + XT_BN - 1) / XT_BN - first_block : 0;
     const int share = (blocks_all + cluster - 1) / cluster;
     const int block0 = first_block + rank * share, nblk = max(0, min(share, blocks_all - rank * share));
-    float m_used = -INFINITY, l_run = 0.0f;
 
-    if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-        if (warp == 8 || warp == 9) {
+    const int role = warp_same(warp);                               // (the branches are then the same in all lanes for the compiler too: see elect_one)
+    if (role >= 8) {
+        if (role == 8 || role == 9) {
             // ---- the loaders: a lane a box (a page's rows of one panel), as soon as the block's buffer is free; where the boxes lie is looked up a block ahead ----
-            const bool keys = warp == 8;
+            const bool keys = role == 8;
             const CUtensorMap* map = keys ? &map_k : &map_v;
             uint64_t* full = keys ? k_full : v_full;
             uint64_t* freed = keys ? k_free : v_free;
-            const int page = 1 << a.page_shift, boxes = XT_BN >> a.page_shift, box = lane % boxes, panel = lane / boxes;
+            const int page = 1 << a.page_shift, rows = min(page, XT_BN), boxes = XT_BN / rows, box = lane % boxes, panel = lane / boxes;
             const bool loads = panel < NH;
             auto row_of = [&](int i) -> int {                       // the box's first row among the cache's rows (past them: zeros)
-                const int key = (block0 + i) * XT_BN + box * page;
+                const int key = (block0 + i) * XT_BN + box * rows;
                 if (!loads || i >= nblk || key >= len) return arg.cache_rows;
-                return (int)(((unsigned)table[key >> a.page_shift] * (unsigned)a.K + (unsigned)kh) << a.page_shift);
+                return (int)((((unsigned)table[key >> a.page_shift] * (unsigned)a.K + (unsigned)kh) << a.page_shift) + (unsigned)(key & (page - 1)));
             };
             if (keys && nblk > 0 && lane < NH * (two ? 2 : 1)) {
                 const int t = lane / NH, p = lane % NH;
@@ -240,21 +270,21 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
                 tma_load_3d(sQ + t * XT_TILE + p * (XT_BM * 128), &map_q, p * 64, kh * G, tok0 + t * per_tile, q_full);
             }
             __syncwarp();
-            int row = row_of(0);
+            int from_row = row_of(0);
             bool ok = true;
             int asked = 0;
             for (int i = 0; ok && i < nblk; ++i) {
                 const int st = i % XT_STAGES;
                 if (i >= XT_STAGES) ok = warp_wait(&freed[st], ((i / XT_STAGES) - 1) & 1, abort, error_flag, 41);
                 if (!ok) break;
-                uint8_t* dst = (keys ? sK : sV) + st * XT_TILE;
-                // the page that the source ends in: its values by plain stores, zeros from there on
-                const int tail = keys ? 0 : len - (block0 + i) * XT_BN, cut = tail > 0 && tail < XT_BN ? tail >> a.page_shift : XT_BN;
-                const bool partial = cut < XT_BN && (tail & (page - 1)) != 0;
+                uint8_t* dst = (keys ? sK : sV) + st * XT_KV;
+                // the box that the source ends in: its values by plain stores, zeros from there on
+                const int tail = keys ? XT_BN : len - (block0 + i) * XT_BN, cut = tail < XT_BN ? tail / rows : boxes;
+                const bool partial = cut < boxes && tail % rows != 0;
                 if (partial) {
-                    const bf16* src = cross_row<bf16>(a, a.v_cache, table, kh, (block0 + i) * XT_BN + cut * page);
-                    for (int x = lane; x < page * NH * 8; x += 32) {
-                        const int rw = x / (NH * 8), c = x % (NH * 8), at = cut * page + rw;
+                    const bf16* src = cross_row<bf16>(a, a.v_cache, table, kh, (block0 + i) * XT_BN + cut * rows);
+                    for (int x = lane; x < rows * NH * 8; x += 32) {
+                        const int rw = x / (NH * 8), c = x % (NH * 8), at = cut * rows + rw;
                         uint4 v = make_uint4(0, 0, 0, 0);
                         if (at < tail && c * 8 < D) v = *reinterpret_cast<const uint4*>(src + (size_t)rw * D + c * 8);
                         *reinterpret_cast<uint4*>(dst + (c >> 3) * (XT_BN * 128) + at * 128 + (((c & 7) ^ (at & 7)) << 4)) = v;
@@ -262,87 +292,84 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                 }
-                if (lane == 0) mbar_expect_tx(&full[st], (uint32_t)(XT_TILE - (partial ? NH * page * 128 : 0)));
+                if (lane == 0) mbar_expect_tx(&full[st], (uint32_t)(XT_KV - (partial ? NH * rows * 128 : 0)));
                 __syncwarp();
-                if (loads && !(partial && box == cut)) tma_load_2d(dst + panel * (XT_BN * 128) + box * page * 128, map, panel * 64, row, &full[st]);
-                row = row_of(i + 1);
+                if (loads && !(partial && box == cut)) tma_load_2d(dst + panel * (XT_BN * 128) + box * rows * 128, map, panel * 64, from_row, &full[st]);
+                from_row = row_of(i + 1);
                 asked = i + 1;
             }
             // (what was asked for has to land before the block ends; where all went well the issuer has waited for it)
             if (!ok)
                 for (int i = max(0, asked - XT_STAGES); i < asked; ++i) mbar_wait_warp(&full[i % XT_STAGES], (i / XT_STAGES) & 1);
-        } else if (warp == 10) {
-            // ---- the issuer ----
+        } else {
+            // ---- the issuers, one a tile: what one spends on its barriers is time in which the other's products run ----
             constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(XT_BN >> 3) << 17) | ((uint32_t)(XT_BM >> 4) << 24);
             constexpr uint32_t idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(XT_BM >> 4) << 24);
-            const uint32_t elected = elect_one(), tmem = warp_same(tmem_base);
-            const int blocks = warp_same(nblk);
-            const int tiles = warp_same(two ? 2 : 1);
-            auto scores = [&](int t, int i) {
-                const uint64_t qdesc = umma_desc(smem_u32(sQ + t * XT_TILE)), kdesc = umma_desc(smem_u32(sK + (i % XT_STAGES) * XT_TILE));
+            const uint32_t elected = elect_one(), t = (uint32_t)(role - 10), tmem = warp_same(tmem_base);
+            const uint32_t tmem_s = tmem + t * 128, tmem_o = tmem + XT_O_COL + t * 128;
+            const int both = warp_same((int)two), blocks = both ? warp_same(nblk) : (warp_same(nblk) + 1 - (int)t) >> 1;
+            auto block = [&](int i) { return both ? i : 2 * i + (int)t; };    // number i of this issuer's blocks
+            uint64_t *s_bar = s_full + 2 * t, *p_bar = p_full + 2 * t, *o_bar = o_done + 2 * t;
+            const uint64_t qdesc = umma_desc(smem_u32(sQ) + (both ? t * XT_TILE : 0u));
+            auto scores = [&](int i) {
+                const int st = block(i) % XT_STAGES;
+                const uint64_t kdesc = umma_desc(smem_u32(sK) + st * XT_KV);
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t step = (uint32_t)((kk / 4) * (128 * 128 >> 4) + 2 * (kk % 4));
-                    umma_bf16(tmem + (uint32_t)(t * XT_BN), qdesc + step, kdesc + step, idesc_s, kk > 0 ? 1u : 0u, elected);
-                }
-                umma_commit(&s_full[t], elected);
+                for (int kk = 0; kk < D / 16; ++kk)
+                    umma_bf16(tmem_s + (uint32_t)((i & 1) * XT_BN), qdesc + (uint32_t)((kk / 4) * (XT_BM * 128 >> 4) + 2 * (kk % 4)),
+                              kdesc + (uint32_t)((kk / 4) * (XT_BN * 128 >> 4) + 2 * (kk % 4)), idesc_s, kk > 0 ? 1u : 0u, elected);
+                umma_commit(&s_bar[i & 1], elected);
+                umma_commit(&k_free[st], elected);
             };
-            auto values = [&](int t, int i) {
-                const uint64_t vdesc = umma_desc_mn(smem_u32(sV + (i % XT_STAGES) * XT_TILE), XT_BN * 128);
-#pragma unroll
-                for (int kk = 0; kk < XT_BN / 16; ++kk)
-                    umma_bf16_tmem_a(tmem + (uint32_t)(2 * XT_BN + t * 128), tmem + (uint32_t)(t * XT_BN + kk * 8), vdesc + (uint32_t)(kk * (2048 >> 4)), idesc_pv,
-                                     (i > 0 || kk > 0) ? 1u : 0u, elected);
-            };
-            bool ok = blocks > 0 && warp_wait(q_full, 0, abort, error_flag, 42) && warp_wait(&k_full[0], 0, abort, error_flag, 42);
-            if (ok) {
+            bool ok = blocks > 0 && warp_wait(q_full, 0, abort, error_flag, 42);
+            for (int i = 0; ok && i < min(2, blocks); ++i) {
+                ok = warp_wait(&k_full[block(i) % XT_STAGES], (block(i) / XT_STAGES) & 1, abort, error_flag, 42);
+                if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                for (int t = 0; t < tiles; ++t) scores(t, 0);
-                umma_commit(&k_free[0], elected);
+                scores(i);
             }
             for (int i = 0; ok && i < blocks; ++i) {
-                const int st = i % XT_STAGES, nx = (i + 1) % XT_STAGES;
-                ok = warp_wait(&v_full[st], (i / XT_STAGES) & 1, abort, error_flag, 43);
-                for (int t = 0; ok && t < tiles; ++t) {
-                    ok = warp_wait(&p_full[t], i & 1, abort, error_flag, 44);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    values(t, i);
-                    if (t == tiles - 1) umma_commit(&v_free[st], elected);
-                    if (i + 1 < blocks) {
-                        // (S goes where P lies: the tensor core takes the products in the order they were issued)
-                        if (t == 0) ok = warp_wait(&k_full[nx], ((i + 1) / XT_STAGES) & 1, abort, error_flag, 45);
-                        if (!ok) break;
-                        scores(t, i + 1);
-                        if (t == tiles - 1) umma_commit(&k_free[nx], elected);
-                    } else {
-                        umma_commit(&o_done[t], elected);
-                    }
-                }
+                const int st = block(i) % XT_STAGES, next = block(i + 2);
+                const bool more = i + 2 < blocks;
+                ok = warp_wait(&v_full[st], (block(i) / XT_STAGES) & 1, abort, error_flag, 43);
+                if (ok && more) ok = warp_wait(&k_full[next % XT_STAGES], (next / XT_STAGES) & 1, abort, error_flag, 45);
+                if (ok) ok = warp_wait(&p_bar[i & 1], (i >> 1) & 1, abort, error_flag, 44);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint64_t vdesc = umma_desc_mn(smem_u32(sV) + st * XT_KV, XT_BN * 128);
+#pragma unroll
+                for (int kk = 0; kk < XT_BN / 16; ++kk)
+                    umma_bf16_tmem_a(tmem_o, tmem_s + (uint32_t)((i & 1) * XT_BN + kk * 8), vdesc + (uint32_t)(kk * (2048 >> 4)), idesc_pv, (i > 0 || kk > 0) ? 1u : 0u, elected);
+                if (more) scores(i + 2);                            // (S goes where P lies: the tensor core takes an issuer's products in their order)
+                umma_commit(&o_bar[i & 1], elected);
+                umma_commit(&v_free[st], elected);
             }
             if (!ok && blocks > 0) {                                // (and what was issued has to end)
-                umma_commit(drained, elected);
-                mbar_wait_warp(drained, 0);
+                umma_commit(&drained[t], elected);
+                mbar_wait_warp(&drained[t], 0);
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         // ---- the rows ----
         const uint32_t lane_base = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
-        const uint32_t s_col = lane_base + (uint32_t)(tile * XT_BN), o_col = lane_base + (uint32_t)(2 * XT_BN + tile * 128);
+        const uint32_t o_col = lane_base + (uint32_t)(XT_O_COL + tile * 128);
         const float sl2 = a.scale * 1.4426950408889634f;
+        // (rows that are not there or see nothing: their results are not looked at, so their scores need no mask)
+        const int mask_from = range.y > range.x ? range.x : -0x40000000, mask_to = range.y > range.x ? range.y : 0x7fffffff;
+        float m_used = -INFINITY, l_run = 0.0f;
         bool ok = true;
-        const int steps = tile == 0 || two ? nblk : 0;
+        const int steps = two ? nblk : (nblk + 1 - tile) >> 1;
         for (int i = 0; i < steps; ++i) {
-            ok = warp_wait(&s_full[tile], i & 1, abort, error_flag, 46);
+            const uint32_t s_col = lane_base + (uint32_t)(tile * 128 + (i & 1) * XT_BN);
+            ok = warp_wait(&s_full[tile * 2 + (i & 1)], (i >> 1) & 1, abort, error_flag, 46);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             float s[XT_BN];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld32_async(s_col + c * 32, s + c * 32);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld_wait(s + c * 32);
-            const int key0 = (block0 + i) * XT_BN, from = range.x - key0, to = range.y - key0;
+            tmem_ld32_async(s_col, s);
+            tmem_ld32_async(s_col + 32, s + 32);
+            tmem_ld_wait(s);
+            tmem_ld_wait(s + 32);
+            const int key0 = (block0 + (two ? i : 2 * i + tile)) * XT_BN, from = mask_from - key0, to = mask_to - key0;
             if (__any_sync(0xffffffffu, from > 0 || to < XT_BN)) {
 #pragma unroll
                 for (int j = 0; j < XT_BN; ++j)
@@ -353,55 +380,64 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
             for (int j = 0; j < XT_BN; j += 8)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) m4[e] = max3(m4[e], s[j + 2 * e], s[j + 2 * e + 1]);
-            const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-            const float m_true = fmaxf(m_used, mx * sl2);
+            const float m_true = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sl2;
+            float corr = 1.0f;
             const bool raise = m_true > m_used + 8.0f || (m_used == -INFINITY && m_true != -INFINITY);
-            const float m_new = raise ? m_true : m_used;
-            const float corr = raise ? xt_exp2(m_used - m_new) : 1.0f;
-            if (i > 0 && __any_sync(0xffffffffu, raise)) {          // (P V of the blocks ahead is done: these scores were issued after it)
+            if (__any_sync(0xffffffffu, raise)) {
+                if (raise) { corr = xt_exp2(m_used - m_true); m_used = m_true; }
+                if (i > 0) {                                        // (P V of the blocks ahead has to be done; of the one before last it is, these scores came after it)
+                    ok = warp_wait(&o_done[tile * 2 + ((i - 1) & 1)], ((i - 1) >> 1) & 1, abort, error_flag, 47);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-                for (int c = 0; c < D / 16; ++c) {
-                    float o[16];
-                    tmem_ld16(o_col + c * 16, o);
+                    for (int c = 0; c < D / 16; ++c) {
+                        float o[16];
+                        tmem_ld16(o_col + c * 16, o);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) o[j] *= corr;
-                    tmem_st16(o_col + c * 16, o);
+                        for (int j = 0; j < 16; ++j) o[j] *= corr;
+                        tmem_st16(o_col + c * 16, o);
+                    }
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 }
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             }
-            m_used = m_new;
             const float base = m_used == -INFINITY ? 0.0f : m_used;
             const uint64_t scale2 = pair_of(sl2, sl2), base2 = pair_of(-base, -base);
             uint64_t sum2[2] = {0, 0};
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t packed[32];
+            for (int c = 0; c < XT_BN / 32; ++c) {
+                uint32_t packed[16];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const uint64_t x = fma_pair(pair_of(s[c * 64 + 2 * j], s[c * 64 + 2 * j + 1]), scale2, base2);
-                    float x0, x1;
-                    of_pair(x, x0, x1);
-                    const float p0 = xt_exp2(x0), p1 = xt_exp2(x1);
+                for (int j = 0; j < 16; ++j) {
+                    const uint64_t x = fma_pair(pair_of(s[c * 32 + 2 * j], s[c * 32 + 2 * j + 1]), scale2, base2);
+                    float p0, p1;
+                    if ((j & 7) >= 8 - XT_POLY) {
+                        exp2_pair_poly(x, p0, p1);
+                    } else {
+                        of_pair(x, p0, p1);
+                        p0 = xt_exp2(p0); p1 = xt_exp2(p1);
+                    }
                     sum2[j & 1] = add_pair(sum2[j & 1], pair_of(p0, p1));
                     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(packed[j]) : "f"(p1), "f"(p0));
                 }
-                tmem_st32_bits(s_col + c * 32, packed);
+                tmem_st16_bits(s_col + c * 16, packed);
             }
-            float u0, u1;
-            of_pair(add_pair(sum2[0], sum2[1]), u0, u1);
-            l_run = l_run * corr + (u0 + u1);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[tile]);
+            if (lane == 0) mbar_arrive(&p_full[tile * 2 + (i & 1)]);
+            float u0, u1;
+            of_pair(add_pair(sum2[0], sum2[1]), u0, u1);
+            l_run = l_run * corr + (u0 + u1);
         }
-        if (ok && steps > 0) ok = warp_wait(&o_done[tile], 0, abort, error_flag, 47);
+        // (the polynomial makes a large number of a NaN: no sum of weights of at most 2^8 comes near it)
+        if (!(l_run < 1.0e30f)) l_run = __int_as_float(0x7fc00000);
+        if (ok && steps > 0) ok = warp_wait(&o_done[tile * 2 + ((steps - 1) & 1)], ((steps - 1) >> 1) & 1, abort, error_flag, 47);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (cluster == 1) {
+        if (cluster == 1 && two) {
             bf16* dst = (bf16*)a.out + ((size_t)(tok0 + my_tok) * a.K * G + my_head) * D;
             const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
             bool odd = false;
-            if (ok && (tile == 0 || two)) {
+            if (ok) {
 #pragma unroll
                 for (int c = 0; c < D / 16; ++c) {
                     float o[16];
@@ -420,23 +456,23 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
                 }
                 if (a.spans != nullptr) {
                     unsigned which = __ballot_sync(0xffffffffu, odd);
-                    while (which != 0) {
+                    for (; which != 0; which &= which - 1) {
                         const int src = __ffs(which) - 1;
-                        which &= which - 1;
                         const int tok = __shfl_sync(0xffffffffu, my_tok, src), head = __shfl_sync(0xffffffffu, my_head, src);
                         const int2 rg = make_int2(__shfl_sync(0xffffffffu, range.x, src), __shfl_sync(0xffffffffu, range.y, src));
                         __syncwarp();
-                        cross_row_alone<bf16>(a, tok0 + tok, head, r, rg);
+                        cross_row_alone<bf16>(arg.a, tok0 + tok, head, r, rg);
                     }
                 }
             }
         } else {
-            // partial results into the tiles' memory, once every product of both tiles is done
-            if (ok && two && nblk > 0) ok = warp_wait(&o_done[1 - tile], 0, abort, error_flag, 47);
+            // partial results into the tiles' memory, once every product of both halves is done
+            const int others = two ? nblk : (nblk + tile) >> 1;
+            if (ok && others > 0) ok = warp_wait(&o_done[(1 - tile) * 2 + ((others - 1) & 1)], ((others - 1) >> 1) & 1, abort, error_flag, 47);
             asm volatile("bar.sync 1, 256;" ::: "memory");
             float* sO = (float*)smem + (size_t)tid * XT_OLD;
             s_m[tid] = m_used; s_l[tid] = l_run;
-            if (ok && (tile == 0 || two)) {
+            if (ok) {
 #pragma unroll
                 for (int c = 0; c < D / 16; ++c) {
                     float o[16];
@@ -455,38 +491,42 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (warp == 0) { __syncwarp(); tmem_free<false>(tmem_base, XT_TMEM); }
-    if (cluster > 1) {
-        cross_cluster_sync();
-        // block `rank` finishes rows rank, rank + cluster, ...: a warp a row, the partial results in rank order
+    if (cluster > 1 || !two) {
+        if (cluster > 1) cross_cluster_sync();
+        // block `rank` finishes rows rank, rank + cluster, ...: a warp a row, the partial results in the order of ranks, and of A and B where both have the row
+        const int parts = two ? 1 : 2, rows = two ? 2 * XT_BM : XT_BM;
+        auto peer = [&](const float* at, int c) { return cluster > 1 ? cross_peer(smem_u32(at), c) : *at; };
         const float* sO = (const float*)smem;
-        for (int row = rank + warp * cluster; row < 2 * XT_BM; row += (XT_THREADS / 32) * cluster) {
-            const int in = row & (XT_BM - 1), tok = (row / XT_BM) * per_tile + in / G, head = kh * G + in % G;
+        for (int done = rank + warp * cluster; done < rows; done += (XT_THREADS / 32) * cluster) {
+            const int in = done & (XT_BM - 1), tok = (done / XT_BM) * per_tile + in / G, head = kh * G + in % G;
             if (in >= per_tile * G || tok >= left) continue;
-            float w[XT_MAX_CLUSTER], top = -INFINITY, sum = 0.0f;
-#pragma unroll
-            for (int c = 0; c < XT_MAX_CLUSTER; ++c) {
-                w[c] = c < cluster ? cross_peer(smem_u32(&s_m[row]), c) : -INFINITY;
-                top = fmaxf(top, w[c]);
-            }
+            float top = -INFINITY, sum = 0.0f, v[(D + 31) / 32];
+            for (int c = 0; c < cluster; ++c)
+                for (int h = 0; h < parts; ++h) top = fmaxf(top, peer(&s_m[done + h * XT_BM], c));
             const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-            for (int c = 0; c < XT_MAX_CLUSTER; ++c)
-                if (c < cluster) { w[c] = xt_exp2(w[c] - base); sum += w[c] * cross_peer(smem_u32(&s_l[row]), c); }
-            const int2 rg = s_range[row];
+            for (int x = 0; x < (D + 31) / 32; ++x) v[x] = 0.0f;
+            for (int c = 0; c < cluster; ++c)
+                for (int h = 0; h < parts; ++h) {
+                    const int at = done + h * XT_BM;
+                    const float w = xt_exp2(peer(&s_m[at], c) - base);
+                    sum = fmaf(w, peer(&s_l[at], c), sum);
+#pragma unroll
+                    for (int x = 0; x < (D + 31) / 32; ++x)
+                        if (x * 32 + lane < D) v[x] = fmaf(w, peer(sO + (size_t)at * XT_OLD + x * 32 + lane, c), v[x]);
+                }
+            const int2 rg = s_range[done];
             bf16* dst = (bf16*)a.out + ((size_t)(tok0 + tok) * a.K * G + head) * D;
             bool odd = false;
-            for (int x = lane; x < D; x += 32) {
-                float v = 0.0f;
 #pragma unroll
-                for (int c = 0; c < XT_MAX_CLUSTER; ++c)
-                    if (c < cluster) v = fmaf(w[c], cross_peer(smem_u32(sO + (size_t)row * XT_OLD + x), c), v);
-                v = rg.y > rg.x && sum != 0.0f ? v / sum : 0.0f;
-                odd |= !(fabsf(v) <= 3.0e38f);
-                dst[x] = __float2bfloat16_rn(v);
+            for (int x = 0; x < (D + 31) / 32; ++x) {
+                const float out = rg.y > rg.x && sum != 0.0f ? v[x] / sum : 0.0f;
+                odd |= !(fabsf(out) <= 3.0e38f);
+                if (x * 32 + lane < D) dst[x * 32 + lane] = __float2bfloat16_rn(out);
             }
-            if (a.spans != nullptr && __any_sync(0xffffffffu, odd)) { __syncwarp(); cross_row_alone<bf16>(a, tok0 + tok, head, r, rg); }
+            if (a.spans != nullptr && __any_sync(0xffffffffu, odd)) { __syncwarp(); cross_row_alone<bf16>(arg.a, tok0 + tok, head, r, rg); }
         }
-        cross_cluster_sync();                                       // (a block's shared memory is read until here)
+        if (cluster > 1) cross_cluster_sync();                      // (a block's shared memory is read until here)
     }
 }
 
@@ -535,9 +575,10 @@ MB_API int mb_attention_cross_tc(const void* q, long long q_stride, const void* 
     int rc = allowed.allow(attention_cross_tc_kernel, XT_SMEM);
     if (rc != 0) return rc;
     CUtensorMap mq, mk, mv;
+    const int box_rows = page_size < XT_BN ? page_size : XT_BN;
     if ((rc = map_queries(&mq, q, q_stride, H, tokens, G, per_tile)) != 0) return rc;
-    if ((rc = map_rows(&mk, k_cache, (uint64_t)cache_rows, (uint32_t)page_size)) != 0) return rc;
-    if ((rc = map_rows(&mv, v_cache, (uint64_t)cache_rows, (uint32_t)page_size)) != 0) return rc;
+    if ((rc = map_rows(&mk, k_cache, (uint64_t)cache_rows, (uint32_t)box_rows)) != 0) return rc;
+    if ((rc = map_rows(&mv, v_cache, (uint64_t)cache_rows, (uint32_t)box_rows)) != 0) return rc;
     const CrossTc arg = {{q, k_cache, v_cache, out, block_table, lens, cu_tokens, spans, q_stride, max_pages, K, G, D, shift, scale}, error_flag, first_request, (int)pairs,
                          (int)cache_rows};
     return launch_kernel(attention_cross_tc_kernel, dim3((unsigned)(requests * pairs), K, chunks), dim3(XT_THREADS), XT_SMEM, s, chunks, mq, mk, mv, arg);
