@@ -1,0 +1,237 @@
+// Attention of single tokens to an encoder's states, bfloat16, up to eight query heads a kv head, pages of at least 16 positions (the formula:
+// cross_common.cuh).  Compiled per head size (-DHEAD_DIM, a multiple of 16 up to 128).
+//
+// Every key and value of a request is read once for all heads of its kv head, so the bytes bound it.  A cluster of up to eight blocks takes one request and kv
+// head, each block an equal run of the positions (requests of a batch have sources of all lengths: shares by length keep the blocks of a cluster equal, where runs
+// of a fixed length leave most blocks of short ones idle); its four warps take stages of 16 positions in turn, each through a ring of its own (cp.async into padded
+// rows, three stages on their way a warp: 96 KB an SM's block), no barrier of the block in the loop.  The query heads are rows 0..7 of mma.sync.m16n8k16:
+//   S = Q K^T   rows 8..15 of Q are zeros;
+//   O = P V     rows 0..7 hold a weight rounded to bfloat16, rows 8..15 what the rounding took off, rounded in turn: O's rows r and r + 8 add up to the weights'
+//               product at 16 bits of a weight, for no more products.
+// Maximum, sum and O are float32; warps, then blocks (in shared memory, rank order), add up theirs scaled to the common maximum.
+// Positions outside the row's range are zeros in shared memory (asked for with no bytes), so what lies there does not matter.
+#define MB_LIB "attention_cross_decode"
+#define MB_LIB_ID 44
+#include "cross_common.cuh"
+#include "mma_helpers.cuh"
+
+#ifndef HEAD_DIM
+#error "compile with -DHEAD_DIM=<multiple of 16, at most 128>"
+#endif
+static_assert(HEAD_DIM % 16 == 0 && HEAD_DIM >= 16 && HEAD_DIM <= 128, "heads in steps of 16 up to 128");
+
+#define D HEAD_DIM
+#define XD_WARPS 4
+#define XD_KEYS 16                               // positions of a stage
+#ifndef XD_STAGES
+#define XD_STAGES 3
+#endif
+#define XD_LD (D + 8)                            // elements of a padded row: ldmatrix without bank conflicts
+#define XD_STAGE_BYTES (2 * XD_KEYS * XD_LD * 2)
+#define XD_RING (XD_STAGES * XD_STAGE_BYTES)
+#define XD_SMEM (XD_WARPS * XD_RING)
+#define XD_MAX_CLUSTER 8
+static_assert(8 * D * 4 <= XD_RING, "a warp's O is written over its ring");
+
+__device__ __forceinline__ float xd_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void cp_async16_or_zeros(void* dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
+__global__ void __launch_bounds__(XD_WARPS * 32) attention_cross_decode_kernel(CrossArgs a, int first_request) {
+    extern __shared__ __align__(16) uint8_t xd_smem[];
+    __shared__ float w_m[XD_WARPS][8], w_l[XD_WARPS][8], c_m[8], c_l[8];
+    __shared__ __align__(16) float c_o[8 * D];
+    PDL_ENTER();
+    a.q = pdl_fresh((const char*)a.q); a.k_cache = pdl_fresh((const char*)a.k_cache); a.v_cache = pdl_fresh((const char*)a.v_cache);
+    a.block_table = pdl_fresh(a.block_table); a.lens = pdl_fresh(a.lens); a.cu_tokens = pdl_fresh(a.cu_tokens); a.spans = pdl_fresh(a.spans);
+    const int r = first_request + blockIdx.x, kh = blockIdx.y, rank = blockIdx.z, cluster = gridDim.z, G = a.G;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int t = a.cu_tokens[r], len = max(0, min(a.lens[r], a.max_pages << a.page_shift));
+    const int2 range = cross_range(a, t, len);
+    const int* table = a.block_table + (size_t)r * a.max_pages;
+    // stages of 16 positions: the block's share, and of it every fourth for this warp
+    const int stage0 = range.x / XD_KEYS, stages = range.y > range.x ? (range.y + XD_KEYS - 1) / XD_KEYS - stage0 : 0;
+    const int share = (stages + cluster - 1) / cluster, mine0 = stage0 + rank * share, mine_n = max(0, min(share, stages - rank * share));
+    const int steps = mine_n > warp ? (mine_n - warp + XD_WARPS - 1) / XD_WARPS : 0;
+
+    // the query rows straight into the MMA's A fragments: lane l holds row l / 4, columns 2 (l % 4) + {0, 1} and + 8 of every 16
+    uint32_t qa[D / 16][4];
+    {
+        const int row = lane >> 2;
+        const bf16* q = (const bf16*)a.q + (size_t)t * a.q_stride + (size_t)(kh * G + (row < G ? row : 0)) * D + 2 * (lane & 3);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+            qa[kk][0] = row < G ? *reinterpret_cast<const uint32_t*>(q + kk * 16) : 0u;
+            qa[kk][2] = row < G ? *reinterpret_cast<const uint32_t*>(q + kk * 16 + 8) : 0u;
+            qa[kk][1] = qa[kk][3] = 0u;
+        }
+    }
+    uint8_t* ring = xd_smem + (size_t)warp * XD_RING;
+    const size_t head_rows = (size_t)kh << a.page_shift, page_rows = (size_t)a.K << a.page_shift;
+    // page of step i, for the 32 steps around: a lane a step
+    int pages = 0;
+    auto look_up = [&](int i) {
+        const int step = i + lane;
+        pages = step < steps ? table[((mine0 + warp + step * XD_WARPS) * XD_KEYS) >> a.page_shift] : 0;
+    };
+    auto issue = [&](int i) {
+        if (i < steps) {
+            if ((i & 31) == 0) look_up(i);
+            const int key0 = (mine0 + warp + i * XD_WARPS) * XD_KEYS;
+            const size_t row0 = (size_t)__shfl_sync(0xffffffffu, pages, i & 31) * page_rows + head_rows + (size_t)(key0 & ((1 << a.page_shift) - 1));
+            const bf16 *ks = (const bf16*)a.k_cache + row0 * D, *vs = (const bf16*)a.v_cache + row0 * D;
+            bf16* dst = reinterpret_cast<bf16*>(ring + (size_t)(i % XD_STAGES) * XD_STAGE_BYTES);
+            constexpr int PIECES = D / 8;
+#pragma unroll
+            for (int x = lane; x < XD_KEYS * PIECES; x += 32) {
+                const int row = x / PIECES, piece = x % PIECES;
+                const bool there = key0 + row >= range.x && key0 + row < range.y;
+                cp_async16_or_zeros(dst + row * XD_LD + piece * 8, ks + row * D + piece * 8, there);
+                cp_async16_or_zeros(dst + (XD_KEYS + row) * XD_LD + piece * 8, vs + row * D + piece * 8, there);
+            }
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < XD_STAGES; ++i) issue(i);
+
+    const float sl2 = a.scale * 1.4426950408889634f;
+    float m = -INFINITY, l = 0.0f;                                  // of this lane's row (query head lane / 4)
+    float o[D / 8][4];                                              // [0], [1]: row lane / 4; [2], [3]: what the rounded weights left
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+    for (int i = 0; i < steps; ++i) {
+        cp_async_wait<XD_STAGES - 1>();
+        __syncwarp();
+        const int key0 = (mine0 + warp + i * XD_WARPS) * XD_KEYS;
+        const bf16* sK = reinterpret_cast<const bf16*>(ring + (size_t)(i % XD_STAGES) * XD_STAGE_BYTES);
+        const bf16* sV = sK + XD_KEYS * XD_LD;
+        float sc[2][4];
+        sc[0][0] = sc[0][1] = sc[0][2] = sc[0][3] = sc[1][0] = sc[1][1] = sc[1][2] = sc[1][3] = 0.0f;
+        const uint32_t k_addr = (uint32_t)__cvta_generic_to_shared(sK + ((lane & 7) + (lane >> 4) * 8) * XD_LD + ((lane >> 3) & 1) * 8);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+            uint32_t b0, b1, b2, b3;
+            ldsm_x4(k_addr + kk * 32, b0, b1, b2, b3);
+            mma_bf16_16816(sc[0], qa[kk], b0, b1);
+            mma_bf16_16816(sc[1], qa[kk], b2, b3);
+        }
+        float s[4] = {sc[0][0] * sl2, sc[0][1] * sl2, sc[1][0] * sl2, sc[1][1] * sl2};
+        if (key0 < range.x || key0 + XD_KEYS > range.y) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int key = key0 + 2 * (lane & 3) + (j >> 1) * 8 + (j & 1);
+                if (key < range.x || key >= range.y) s[j] = -INFINITY;
+            }
+        }
+        float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        if (__any_sync(0xffffffffu, mx > m)) {                      // (seldom after the first stages)
+            const float m_new = fmaxf(m, mx), corr = xd_exp2(m - (m_new == -INFINITY ? 0.0f : m_new));
+            m = m_new;
+            l *= corr;
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) { o[c][0] *= corr; o[c][1] *= corr; o[c][2] *= corr; o[c][3] *= corr; }
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { s[j] = xd_exp2(s[j] - base); l += s[j]; }
+        uint32_t pa[4];
+        pa[0] = pack_bf16(s[0], s[1]);
+        pa[2] = pack_bf16(s[2], s[3]);
+        const float2 h0 = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&pa[0])), h1 = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&pa[2]));
+        pa[1] = pack_bf16(s[0] - h0.x, s[1] - h0.y);
+        pa[3] = pack_bf16(s[2] - h1.x, s[3] - h1.y);
+        const uint32_t v_addr = (uint32_t)__cvta_generic_to_shared(sV + ((lane & 7) + ((lane >> 3) & 1) * 8) * XD_LD + (lane >> 4) * 8);
+#pragma unroll
+        for (int c = 0; c < D / 8; c += 2) {
+            uint32_t b0, b1, b2, b3;
+            ldsm_x4_trans(v_addr + c * 16, b0, b1, b2, b3);
+            mma_bf16_16816(o[c], pa, b0, b1);
+            mma_bf16_16816(o[c + 1], pa, b2, b3);
+        }
+        __syncwarp();                                               // the stage is free
+        issue(i + XD_STAGES);
+    }
+    cp_async_wait<0>();
+    __syncwarp();
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    {
+        float* mine = reinterpret_cast<float*>(ring) + (lane >> 2) * D + 2 * (lane & 3);
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) *reinterpret_cast<float2*>(mine + c * 8) = make_float2(o[c][0] + o[c][2], o[c][1] + o[c][3]);
+        if ((lane & 3) == 0) { w_m[warp][lane >> 2] = m; w_l[warp][lane >> 2] = l; }
+    }
+    __syncthreads();
+    // the block's result, then the cluster's
+    for (int x = threadIdx.x; x < G * D; x += XD_WARPS * 32) {
+        const int row = x / D;
+        float top = -INFINITY, sum = 0.0f, v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < XD_WARPS; ++w) top = fmaxf(top, w_m[w][row]);
+        const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int w = 0; w < XD_WARPS; ++w) {
+            const float f = xd_exp2(w_m[w][row] - base);
+            sum = fmaf(f, w_l[w][row], sum);
+            v = fmaf(f, reinterpret_cast<const float*>(xd_smem + (size_t)w * XD_RING)[x], v);
+        }
+        if (cluster == 1) {
+            ((bf16*)a.out)[((size_t)t * a.K * G + kh * G) * D + x] = __float2bfloat16_rn(range.y > range.x ? v / sum : 0.0f);
+        } else {
+            c_o[x] = v;
+            if (x % D == 0) { c_m[row] = top; c_l[row] = sum; }
+        }
+    }
+    if (cluster == 1) return;
+    cross_cluster_sync();
+    for (int x = rank * XD_WARPS * 32 + threadIdx.x; x < G * D; x += cluster * XD_WARPS * 32) {
+        const int row = x / D;
+        float f[XD_MAX_CLUSTER], u[XD_MAX_CLUSTER], part[XD_MAX_CLUSTER], top = -INFINITY, sum = 0.0f, v = 0.0f;
+#pragma unroll
+        for (int c = 0; c < XD_MAX_CLUSTER; ++c) {
+            const int from = c < cluster ? c : 0;
+            f[c] = cross_peer((uint32_t)__cvta_generic_to_shared(&c_m[row]), from);
+            u[c] = cross_peer((uint32_t)__cvta_generic_to_shared(&c_l[row]), from);
+            part[c] = cross_peer((uint32_t)__cvta_generic_to_shared(&c_o[x]), from);
+        }
+#pragma unroll
+        for (int c = 0; c < XD_MAX_CLUSTER; ++c) if (c < cluster) top = fmaxf(top, f[c]);
+        const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int c = 0; c < XD_MAX_CLUSTER; ++c)
+            if (c < cluster) {
+                const float w = xd_exp2(f[c] - base);
+                sum = fmaf(w, u[c], sum);
+                v = fmaf(w, part[c], v);
+            }
+        ((bf16*)a.out)[((size_t)t * a.K * G + kh * G) * D + x] = __float2bfloat16_rn(range.y > range.x ? v / sum : 0.0f);
+    }
+    cross_cluster_sync();                                           // (a block's shared memory is read until here)
+}
+
+// Requests first_request .. first_request + requests - 1, one token each.  chunks: 1, 2, 4 or 8 blocks share a request and kv head.
+MB_API int mb_attention_cross_decode(const void* q, long long q_stride, const void* k_cache, const void* v_cache, void* out, const int* block_table, int max_pages,
+                                     const int* lens, const int* cu_tokens, const int* spans, int first_request, int requests, int chunks, int H, int K, int page_size,
+                                     float scale, cudaStream_t s) {
+    if (requests <= 0) return 0;
+    int shift = -1;
+    for (int b = 4; b < 24; ++b)
+        if ((1 << b) == page_size) shift = b;
+    if (shift < 0 || K <= 0 || H <= 0 || H % K != 0 || H / K > 8 || K > 65535 || ((long long)max_pages << shift) > 0x7fffff00LL ||
+        (((uintptr_t)q | (uintptr_t)out) & 3) != 0 || q_stride % 2 != 0 || (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) != 0 ||
+        !(chunks == 1 || chunks == 2 || chunks == 4 || chunks == XD_MAX_CLUSTER))
+        return MB_ERR_BAD_SIZE;
+    static LaunchSmem allowed;
+    const int rc = allowed.allow(attention_cross_decode_kernel, XD_SMEM);
+    if (rc != 0) return rc;
+    const CrossArgs a = {q, k_cache, v_cache, out, block_table, lens, cu_tokens, spans, q_stride, max_pages, K, H / K, D, shift, scale};
+    return launch_kernel(attention_cross_decode_kernel, dim3(requests, K, chunks), dim3(XD_WARPS * 32), XD_SMEM, s, chunks, a, first_request);
+}

@@ -2808,18 +2808,47 @@ def gla_jobs(dtype, d: int, dv: int, rank: int) -> dict:
 
 # ---- a decoder that reads an encoder's states: heads with positions of several axes, the states' pages, attention to them ----
 
-def _on_current_device(*tensors) -> None:
-    """Launches go to the current device's stream: tensors of another device (or of the host) are refused."""
-    here = _current_device() if torch.cuda.is_available() else -1
+def _on_current_device(*tensors) -> int:
+    """The current device: launches go to its current stream, and tensors of another device (or of the host) are refused."""
+    here = None
     for t in tensors:
-        if t is not None and (here < 0 or t.get_device() != here):
-            raise KernelError(f"marin_b200 kernels run on tensors of the current CUDA device ({'none' if here < 0 else here}); there is no CPU path: got one on {t.device}")
+        if t is not None:
+            d = t.get_device()
+            if here is None and d >= 0:
+                here = _current_device()
+            if d != here:
+                raise KernelError(f"marin_b200 kernels run on tensors of the current CUDA device; there is no CPU path: got one on {t.device}")
+    return here
 
 
 def _int32(what: str, *tensors) -> None:
     for t in tensors:
-        if t.dtype != torch.int32 or not t.is_contiguous():
+        if t.dtype is not torch.int32 or not t.is_contiguous():
             raise KernelError(f"{what}: expects contiguous int32 tensors, got {t.dtype}")
+
+
+_entries: dict = {}
+_KINDS = {"p": _c_void_p, "i": _c_int, "l": ctypes.c_longlong, "f": _c_float}
+
+
+def _entry(lib, name: str, kinds: str):
+    """A library's function with its arguments' types said once (p: an address or None, i, l: whole numbers of 32 and 64 bits, f: a float): a call then takes plain
+    Python numbers, half a microsecond an argument less than wrapping each (calls of a few microseconds are bound by the host)."""
+    key = (lib._name, name)
+    fn = _entries.get(key)
+    if fn is None:
+        fn = getattr(lib, name)
+        fn.argtypes = [_KINDS[k] for k in kinds]
+        _entries[key] = fn
+    return fn
+
+
+def _stream_of(device: int):
+    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
+
+
+def _address(t: Optional[torch.Tensor]):
+    return t.data_ptr() if t is not None else None
 
 
 def axis_sections(sections, spread: bool = False) -> list:
@@ -2847,7 +2876,7 @@ def qk_norm_axes_write(rows: torch.Tensor, q_out: Optional[torch.Tensor], q_weig
     ``inv_freq`` float32 ``[rotary_dim / 2]``; the angle in 64 bits); queries go to ``q_out`` ``[T, H * d]``, keys and values into the paged caches at ``slot_mapping``
     (negative: a padded token, nothing is stored).  ``rows`` ``[T, >= (H + 2 K) * d]`` may be columns of wider rows.  ``H = 0`` (``q_out`` None): an encoder's
     keys and values alone; ``write_kv=False``: queries alone.  ``axis_of`` is held to the axes there are, places past the caches store nothing."""
-    _on_current_device(rows, q_out, q_weight, k_weight, positions, axis_of, inv_freq, slot_mapping, k_cache, v_cache)
+    device = _on_current_device(rows, q_out, q_weight, k_weight, positions, axis_of, inv_freq, slot_mapping, k_cache, v_cache)
     if rows.dim() != 2:
         raise KernelError(f"qk_norm_axes_write: rows are [T, columns], got {tuple(rows.shape)}")
     T = rows.shape[0]
@@ -2876,12 +2905,13 @@ def qk_norm_axes_write(rows: torch.Tensor, q_out: Optional[torch.Tensor], q_weig
         cache_rows = k_cache.shape[0] * page_size
     if T == 0:
         return
-    _cost(2 * T * wanted * rows.element_size() + (_size(positions) if inv_freq is not None else 0), 8.0 * T * wanted)
-    _check(_lib("mb_rope_axes").mb_heads_axes(
-        _ptr(rows), _code(rows), ctypes.c_longlong(rows.stride(0)), _ptr(q_out), _ptr(q_weight), _ptr(k_weight), _c_float(eps), _ptr(positions),
-        _c_int(positions.shape[0] if inv_freq is not None else 0), _ptr(axis_of), _ptr(inv_freq), _c_int(rotary_dim if inv_freq is not None else 0), _c_int(int(interleaved)),
-        _ptr(slot_mapping), _ptr(k_cache), _ptr(v_cache), ctypes.c_longlong(cache_rows), _c_int(page_size), _c_int(T), _c_int(H), _c_int(K), _c_int(d),
-        _c_int(int(write_kv)), _stream()), "qk_norm_axes_write")
+    if launch_log is not None:
+        _cost(2 * T * wanted * rows.element_size() + (_size(positions) if inv_freq is not None else 0), 8.0 * T * wanted)
+    turns = inv_freq is not None
+    _check(_entry(_lib("mb_rope_axes"), "mb_heads_axes", "pilpppfpippiipppliiiiiip")(
+        rows.data_ptr(), _code(rows), rows.stride(0), _address(q_out), _address(q_weight), _address(k_weight), eps, _address(positions), positions.shape[0] if turns else 0,
+        _address(axis_of), _address(inv_freq), rotary_dim if turns else 0, int(interleaved), _address(slot_mapping), _address(k_cache), _address(v_cache), cache_rows, page_size,
+        T, H, K, d, int(write_kv), _stream_of(device)), "qk_norm_axes_write")
 
 
 #: most requests of one ``page_step`` (the running sums over them lie in a block's shared memory)
@@ -2899,7 +2929,7 @@ def page_step(before: torch.Tensor, after: torch.Tensor, table: torch.Tensor, fr
 
     All or nothing: where ``left[1]`` is 1 (the free list runs out), 2 (more new tokens than the buffers' room), 3 (a length is negative or longer than a row of the
     table) or 4 (``count`` or what is given back is more than ``free`` holds), no page moves, ``left[0]`` is ``count[0]`` and every token is a padded one."""
-    _on_current_device(before, after, table, free, count, left, cu_tokens, req_index, positions, slots)
+    device = _on_current_device(before, after, table, free, count, left, cu_tokens, req_index, positions, slots)
     _int32("page_step", before, after, table, free, count, left, cu_tokens, req_index, positions, slots)
     R, room = before.numel(), slots.numel()
     if R < 1 or R > PAGE_STEP_REQUESTS:
@@ -2909,10 +2939,11 @@ def page_step(before: torch.Tensor, after: torch.Tensor, table: torch.Tensor, fr
         raise KernelError(f"page_step: after [{R}], table [{R}, columns], count [1], left [2], cu_tokens [{R + 1}] and buffers of one size are wanted")
     if page_size < 1 or page_size & (page_size - 1):
         raise KernelError(f"page_step: page_size {page_size} is no power of two")
-    _cost(4 * (2 * R + R + 1 + 3 * room))
-    _check(_lib("mb_pages").mb_page_step(_ptr(before), _ptr(after), _ptr(table), _ptr(free), _ptr(count), _ptr(left), _ptr(cu_tokens), _ptr(req_index), _ptr(positions),
-                                         _ptr(slots), _c_int(R), _c_int(table.shape[1]), _c_int(free.numel()), _c_int(page_size), _c_int(room), _stream()),
-           "page_step (tensors must not overlap)")
+    if launch_log is not None:
+        _cost(4 * (2 * R + R + 1 + 3 * room))
+    _check(_entry(_lib("mb_pages"), "mb_page_step", "ppppppppppiiiiip")(
+        before.data_ptr(), after.data_ptr(), table.data_ptr(), free.data_ptr(), count.data_ptr(), left.data_ptr(), cu_tokens.data_ptr(), req_index.data_ptr(), positions.data_ptr(),
+        slots.data_ptr(), R, table.shape[1], free.numel(), page_size, room, _stream_of(device)), "page_step (tensors must not overlap)")
 
 
 class Source:
@@ -2927,17 +2958,45 @@ class Source:
 def cross_tc_supported(dtype, H: int, K: int, d: int, page_size: int) -> bool:
     """Whether the tensor-core kernel takes this layout (the others go to the 32-bit one): bfloat16, heads in steps of 16 up to 128, up to 128 query heads a kv
     head, pages of 16 to 128 positions."""
-    return dtype == torch.bfloat16 and d % 16 == 0 and 16 <= d <= 128 and H // K <= 128 and page_size in (16, 32, 64, 128)
+    return dtype is torch.bfloat16 and d % 16 == 0 and 16 <= d <= 128 and H // K <= 128 and page_size in (16, 32, 64, 128)
 
 
-def _cross_tc_lib(d: int):
-    return build.load(f"mb_attention_cross_tc_d{d}", ["attention_cross_tc.cu"], [f"HEAD_DIM={d}"])
+def cross_decode_supported(dtype, H: int, K: int, d: int, page_size: int) -> bool:
+    """Whether single tokens have a kernel of their own: as ``cross_tc_supported`` with up to eight query heads a kv head (rows of a 16-row product whose other half holds
+    what rounding took off the weights) and pages of at least 16."""
+    return dtype is torch.bfloat16 and d % 16 == 0 and 16 <= d <= 128 and H // K <= 8 and page_size >= 16
+
+
+def cross_jobs(dtype, H: int, K: int, d: int, page_size: int) -> dict:
+    """``{library: (sources, defines)}`` of the kernels that ``attention_cross`` runs for this head layout."""
+    jobs = {"mb_attention_cross": (build.LIBRARIES["mb_attention_cross"], [])}
+    if cross_tc_supported(dtype, H, K, d, page_size):
+        jobs[f"mb_attention_cross_tc_d{d}"] = (["attention_cross_tc.cu"], [f"HEAD_DIM={d}"])
+    if cross_decode_supported(dtype, H, K, d, page_size):
+        jobs[f"mb_attention_cross_decode_d{d}"] = (["attention_cross_decode.cu"], [f"HEAD_DIM={d}"])
+    return jobs
+
+
+def _cross_lib(which: str, d: int):
+    name = f"mb_attention_cross_{which}_d{d}"
+    lib = _libraries.get(name)
+    if lib is None:
+        lib = _libraries[name] = build.load(name, [f"attention_cross_{which}.cu"], [f"HEAD_DIM={d}"])
+    return lib
 
 
 def cross_chunks(blocks: int, longest: int) -> int:
     """Over how many blocks of a cluster (1, 2, 4 or 8) a tile pair's keys are cut: as many as fill the SMs, none with fewer than 256 keys."""
     chunks = 1
     while chunks < 8 and blocks * chunks * 2 <= SM_COUNT and chunks * 256 < longest:
+        chunks *= 2
+    return chunks
+
+
+def cross_decode_chunks(pairs: int, longest: int) -> int:
+    """The same for single tokens (``pairs`` requests times kv heads)."""
+    chunks = 1
+    while chunks < 8 and chunks * 128 < longest and (pairs * chunks < 4 * SM_COUNT or chunks * 1024 < longest):
         chunks *= 2
     return chunks
 
@@ -2949,44 +3008,49 @@ def attention_cross(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     including ``spans[t, 1]``; a token that sees nothing gets zeros.  Keys and values lie in pages ``[page, K, page_size, d]`` (a power of two of positions).  Of ``ctx`` it
     takes ``num_requests``, ``num_decode`` (the first requests, one token each), ``max_query_len`` and ``cu_tokens``; rows of ``q`` ``[T, H * d]`` past the last request's
     are not read and those of ``out`` stay as they were.  ``q`` may be columns of wider rows."""
-    table, lens = source.block_table, source.lens
-    _on_current_device(q, k_cache, v_cache, out, table, lens, ctx.cu_tokens, spans)
-    T, R, nd = q.shape[0], ctx.num_requests, ctx.num_decode
-    if H <= 0 or K <= 0 or H % K or q.dim() != 2 or q.shape[1] != H * d or (q.shape[1] > 1 and q.stride(1) != 1) or out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
-        raise KernelError(f"attention_cross: queries and results are [T, {H * d}] of one dtype ({H} heads over {K} of {d}), got {tuple(q.shape)} and {tuple(out.shape)}")
-    if (k_cache.dtype != q.dtype or v_cache.dtype != q.dtype or k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1] != K or k_cache.shape[3] != d
+    table, lens, cu = source.block_table, source.lens, ctx.cu_tokens
+    device = _on_current_device(q, k_cache, v_cache, out, table, lens, cu, spans)
+    R, nd, dtype, shape, cache = ctx.num_requests, ctx.num_decode, q.dtype, q.shape, k_cache.shape
+    if H <= 0 or K <= 0 or H % K or len(shape) != 2 or shape[1] != H * d or out.shape != shape or out.dtype is not dtype or not out.is_contiguous() or (shape[1] > 1 and q.stride(1) != 1):
+        raise KernelError(f"attention_cross: queries and results are [T, {H * d}] of one dtype ({H} heads over {K} of {d}), got {tuple(shape)} and {tuple(out.shape)}")
+    if (k_cache.dtype is not dtype or v_cache.dtype is not dtype or len(cache) != 4 or cache != v_cache.shape or cache[1] != K or cache[3] != d
             or not k_cache.is_contiguous() or not v_cache.is_contiguous()):
-        raise KernelError(f"attention_cross: caches are contiguous {q.dtype} [pages, {K}, page_size, {d}]")
-    page_size = k_cache.shape[2]
+        raise KernelError(f"attention_cross: caches are contiguous {dtype} [pages, {K}, page_size, {d}]")
+    T, pages, page_size = shape[0], cache[0], cache[2]
     if page_size < 1 or page_size & (page_size - 1) or d > 256:
         raise KernelError(f"attention_cross: pages of a power of two of positions and heads of up to 256, got {page_size} and {d}")
-    _int32("attention_cross", table, lens, ctx.cu_tokens)
-    if table.dim() != 2 or table.shape[0] < R or lens.numel() < R or ctx.cu_tokens.numel() < R + 1 or not 0 <= nd <= R:
+    _int32("attention_cross", table, lens, cu)
+    if table.dim() != 2 or table.shape[0] < R or lens.numel() < R or cu.numel() < R + 1 or not 0 <= nd <= R:
         raise KernelError(f"attention_cross: block_table [{R}, pages], lens [{R}] and cu_tokens [{R + 1}] are wanted")
     if spans is not None:
         _int32("attention_cross", spans)
-        if tuple(spans.shape) != (T, 2):
+        if spans.dim() != 2 or spans.shape[0] != T or spans.shape[1] != 2:
             raise KernelError(f"attention_cross: spans are [{T}, 2]")
     if not 0.0 < scale < float("inf"):
         raise KernelError(f"attention_cross: scale is a positive number, got {scale}")
     if T == 0 or R == 0:
         return
-    longest = max(0, int(source.longest))
-    tc = cross_tc_supported(q.dtype, H, K, d, page_size) and q.stride(0) % 8 == 0 and all(x.data_ptr() % 16 == 0 for x in (q, k_cache, v_cache, out)) and k_cache.shape[0] * K * page_size < 0x7fffff00 and k_cache.shape[0] > 0
-    for first, n, most, which in ((0, nd, 1, "decode"), (nd, R - nd, ctx.max_query_len, "portions")):
+    longest, most, columns, stride = max(0, int(source.longest)), ctx.max_query_len, table.shape[1], q.stride(0)
+    addresses = (q.data_ptr(), stride, k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr())
+    where = (table.data_ptr(), columns, lens.data_ptr(), cu.data_ptr(), _address(spans))
+    aligned = stride % 8 == 0 and (addresses[0] | addresses[2] | addresses[3] | addresses[4]) % 16 == 0
+    tc = aligned and cross_tc_supported(dtype, H, K, d, page_size) and 0 < pages * K * page_size < 0x7fffff00
+    single = aligned and cross_decode_supported(dtype, H, K, d, page_size)
+    stream, group = _stream_of(device), H // K
+    for first, n, most, which in ((0, nd, 1, "decode"), (nd, R - nd, most, "portions")):
         if n <= 0:
             continue
         if launch_log is not None:
             rows, size = (n if which == "decode" else T - nd), q.element_size()
             _cost(size * (2 * rows * H * d + 2 * n * longest * K * d), 4.0 * rows * longest * H * d)
-        if tc:
-            tiles = -(-most * (H // K) // (2 * (128 // (H // K) * (H // K))))
-            _check(_cross_tc_lib(d).mb_attention_cross_tc(
-                _ptr(q), ctypes.c_longlong(q.stride(0)), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(table), _c_int(table.shape[1]), _ptr(lens), _ptr(ctx.cu_tokens),
-                _ptr(spans), _c_int(first), _c_int(n), _c_int(most), _c_int(T), _c_int(cross_chunks(min(n * tiles, n + (T * (H // K)) // 256) * K, longest)), _c_int(H), _c_int(K), _c_int(page_size),
-                ctypes.c_longlong(k_cache.shape[0]), _c_float(scale), _ptr(_scratch_for(q.device).error), _stream()), f"attention_cross ({which}, tensor cores)")
-            continue
-        _check(_lib("mb_attention_cross").mb_attention_cross(
-            _ptr(q), ctypes.c_longlong(q.stride(0)), _ptr(k_cache), _ptr(v_cache), _ptr(out), _code(q), _ptr(table), _c_int(table.shape[1]), _ptr(lens), _ptr(ctx.cu_tokens),
-            _ptr(spans), _c_int(first), _c_int(n), _c_int(most), _c_int(longest), _c_int(H), _c_int(K), _c_int(d), _c_int(page_size), _c_float(scale), _stream()),
-            f"attention_cross ({which})")
+        if single and most == 1:
+            _check(_entry(_cross_lib("decode", d), "mb_attention_cross_decode", "plppppipppiiiiiifp")(
+                *addresses, *where, first, n, cross_decode_chunks(n * K, longest), H, K, page_size, scale, stream), f"attention_cross ({which})")
+        elif tc:
+            pairs = -(-most // (2 * (128 // group)))
+            _check(_entry(_cross_lib("tc", d), "mb_attention_cross_tc", "plppppipppiiiiiiiilfpp")(
+                *addresses, *where, first, n, most, T, cross_chunks(min(n * pairs, n + T * group // 256) * K, longest), H, K, page_size, pages, scale,
+                _scratch_for(q.device).error.data_ptr(), stream), f"attention_cross ({which}, tensor cores)")
+        else:
+            _check(_entry(_lib("mb_attention_cross"), "mb_attention_cross", "plpppipipppiiiiiiiifp")(
+                *addresses, _code(q), *where, first, n, most, longest, H, K, d, page_size, scale, stream), f"attention_cross ({which})")
