@@ -240,27 +240,20 @@ static int launch_cross(const CrossArgs& a, int first_request, int requests, int
                          max_tiles, whole);
 }
 
-// Requests first_request .. first_request + requests - 1, none with more than max_query tokens or a source longer than `longest`.
-MB_API int mb_attention_cross(const void* q, long long q_stride, const void* k_cache, const void* v_cache, void* out, int dtype, const int* block_table, int max_pages,
-                              const int* lens, const int* cu_tokens, const int* spans, int first_request, int requests, int max_query, int longest, int H, int K,
-                              int d, int page_size, float scale, cudaStream_t s) {
-    if (requests <= 0 || max_query <= 0) return 0;
-    if (K <= 0 || H <= 0 || H % K != 0 || d <= 0 || d > 256 || page_size <= 0 || (page_size & (page_size - 1)) != 0 || K > 65535) return MB_ERR_BAD_SIZE;
-    int shift = 0;
-    while ((1 << shift) < page_size) ++shift;
-    if (((long long)max_pages << shift) > 0x7fffffffLL) return MB_ERR_BAD_SIZE;
-    const int G = H / K;
-    const CrossArgs a = {q, k_cache, v_cache, out, block_table, lens, cu_tokens, spans, q_stride, max_pages, K, G, d, shift, scale};
-    const int whole = dtype == MB_F32 && d % 4 == 0 && (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) == 0;
+MB_API int mb_attention_cross(const CrossCall* c, cudaStream_t s) {
+    if (c->requests <= 0 || c->max_query <= 0) return 0;
+    if (!cross_call_fits(c) || c->d > 256) return MB_ERR_BAD_SIZE;
+    const CrossArgs a = cross_args(c);
+    const int whole = c->dtype == MB_F32 && a.d % 4 == 0 && (((uintptr_t)c->k_cache | (uintptr_t)c->v_cache) & 15) == 0;
     // up to 16 rows (single tokens): tiles of 16, a quarter of the multiply-adds that a tile of 64 would spend on rows that are not there
-    const long long rows = (long long)max_query * G;
+    const long long rows = (long long)c->max_query * a.G;
     const int bm = rows <= 16 ? 16 : 64;
     const long long tiles = (rows + bm - 1) / bm;
-    if (tiles * requests > 0x7fffffffLL) return MB_ERR_BAD_SIZE;
-    const int clusters = cross_chunks(longest), dch = (d + 63) / 64;
-#define CX_CASE(T, B, C) return launch_cross<T, B, C>(a, first_request, requests, (int)tiles, clusters, whole, s)
+    if (tiles * c->requests > 0x7fffffffLL) return MB_ERR_BAD_SIZE;
+    const int clusters = cross_chunks(c->longest), dch = (a.d + 63) / 64;
+#define CX_CASE(T, B, C) return launch_cross<T, B, C>(a, c->first, c->requests, (int)tiles, clusters, whole, s)
 #define CX_WIDTHS(T, B) switch (dch) { case 1: CX_CASE(T, B, 1); case 2: CX_CASE(T, B, 2); case 3: CX_CASE(T, B, 3); default: CX_CASE(T, B, 4); }
-    if (dtype == MB_F32) { if (bm == 16) CX_WIDTHS(float, 16) else CX_WIDTHS(float, 64) }
-    if (dtype == MB_BF16) { if (bm == 16) CX_WIDTHS(bf16, 16) else CX_WIDTHS(bf16, 64) }
+    if (c->dtype == MB_F32) { if (bm == 16) CX_WIDTHS(float, 16) else CX_WIDTHS(float, 64) }
+    if (c->dtype == MB_BF16) { if (bm == 16) CX_WIDTHS(bf16, 16) else CX_WIDTHS(bf16, 64) }
     return MB_ERR_BAD_DTYPE;
 }

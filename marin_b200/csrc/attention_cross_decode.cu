@@ -217,21 +217,14 @@ __global__ void __launch_bounds__(XD_WARPS * 32) attention_cross_decode_kernel(C
     cross_cluster_sync();                                           // (a block's shared memory is read until here)
 }
 
-// Requests first_request .. first_request + requests - 1, one token each.  chunks: 1, 2, 4 or 8 blocks share a request and kv head.
-MB_API int mb_attention_cross_decode(const void* q, long long q_stride, const void* k_cache, const void* v_cache, void* out, const int* block_table, int max_pages,
-                                     const int* lens, const int* cu_tokens, const int* spans, int first_request, int requests, int chunks, int H, int K, int page_size,
-                                     float scale, cudaStream_t s) {
-    if (requests <= 0) return 0;
-    int shift = -1;
-    for (int b = 4; b < 24; ++b)
-        if ((1 << b) == page_size) shift = b;
-    if (shift < 0 || K <= 0 || H <= 0 || H % K != 0 || H / K > 8 || K > 65535 || ((long long)max_pages << shift) > 0x7fffff00LL ||
-        (((uintptr_t)q | (uintptr_t)out) & 3) != 0 || q_stride % 2 != 0 || (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) != 0 ||
-        !(chunks == 1 || chunks == 2 || chunks == 4 || chunks == XD_MAX_CLUSTER))
+// Requests of one token each.
+MB_API int mb_attention_cross_decode(const CrossCall* c, cudaStream_t s) {
+    if (c->requests <= 0) return 0;
+    if (!cross_call_fits(c) || c->d != D || c->dtype != MB_BF16 || c->page_size < XD_KEYS || c->H / c->K > 8 || (((uintptr_t)c->q | (uintptr_t)c->out) & 3) != 0 || c->q_stride % 2 != 0 ||
+        (((uintptr_t)c->k_cache | (uintptr_t)c->v_cache) & 15) != 0 || !chunks_fit(c->chunks))
         return MB_ERR_BAD_SIZE;
     static LaunchSmem allowed;
     const int rc = allowed.allow(attention_cross_decode_kernel, XD_SMEM);
     if (rc != 0) return rc;
-    const CrossArgs a = {q, k_cache, v_cache, out, block_table, lens, cu_tokens, spans, q_stride, max_pages, K, H / K, D, shift, scale};
-    return launch_kernel(attention_cross_decode_kernel, dim3(requests, K, chunks), dim3(XD_WARPS * 32), XD_SMEM, s, chunks, a, first_request);
+    return launch_kernel(attention_cross_decode_kernel, dim3(c->requests, c->K, c->chunks), dim3(XD_WARPS * 32), XD_SMEM, s, c->chunks, cross_args(c), c->first);
 }

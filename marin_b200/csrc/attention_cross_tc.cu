@@ -554,32 +554,24 @@ static int map_queries(CUtensorMap* map, const void* q, long long stride, int H,
     return rc == CUDA_SUCCESS ? 0 : 1000 + (int)rc;
 }
 
-// Requests first_request .. first_request + requests - 1 (none with more than max_query tokens) of a step of `tokens` tokens.  chunks: 1, 2, 4 or 8 blocks
-// share a tile pair's keys.  Pages of 16 to 128 positions; q, caches and out at 16 bytes, q_stride in whole 16-byte steps.
-MB_API int mb_attention_cross_tc(const void* q, long long q_stride, const void* k_cache, const void* v_cache, void* out, const int* block_table, int max_pages,
-                                 const int* lens, const int* cu_tokens, const int* spans, int first_request, int requests, int max_query, int tokens, int chunks, int H,
-                                 int K, int page_size, long long cache_pages, float scale, int* error_flag, cudaStream_t s) {
-    if (requests <= 0 || max_query <= 0) return 0;
-    int shift = -1;
-    for (int b = 4; b < 8; ++b)
-        if ((1 << b) == page_size) shift = b;
-    const long long cache_rows = cache_pages * K * page_size;
-    if (shift < 0 || K <= 0 || H <= 0 || H % K != 0 || H / K > XT_BM || K > 65535 || cache_rows <= 0 || cache_rows > 0x7fffff00LL ||
-        ((long long)max_pages << shift) > 0x7fffff00LL || (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15) != 0 || q_stride % 8 != 0 ||
-        !(chunks == 1 || chunks == 2 || chunks == 4 || chunks == XT_MAX_CLUSTER))
+// Pages of 16 to 128 positions; q, caches and out at 16 bytes, q_stride in whole 16-byte steps.
+MB_API int mb_attention_cross_tc(const CrossCall* c, cudaStream_t s) {
+    if (c->requests <= 0 || c->max_query <= 0) return 0;
+    const long long cache_rows = c->cache_pages * c->K * c->page_size;
+    if (!cross_call_fits(c) || c->d != D || c->dtype != MB_BF16 || c->page_size < 16 || c->page_size > 128 || c->H / c->K > XT_BM || cache_rows <= 0 || cache_rows > 0x7fffff00LL ||
+        (((uintptr_t)c->q | (uintptr_t)c->k_cache | (uintptr_t)c->v_cache | (uintptr_t)c->out) & 15) != 0 || c->q_stride % 8 != 0 || !chunks_fit(c->chunks))
         return MB_ERR_BAD_SIZE;
-    const int G = H / K, per_tile = XT_BM / G;
-    const long long pairs = (max_query + 2LL * per_tile - 1) / (2 * per_tile);
-    if (pairs * requests > 0x7fffffffLL) return MB_ERR_BAD_SIZE;
+    const int G = c->H / c->K, per_tile = XT_BM / G;
+    const long long pairs = (c->max_query + 2LL * per_tile - 1) / (2 * per_tile);
+    if (pairs * c->requests > 0x7fffffffLL) return MB_ERR_BAD_SIZE;
     static LaunchSmem allowed;
     int rc = allowed.allow(attention_cross_tc_kernel, XT_SMEM);
     if (rc != 0) return rc;
     CUtensorMap mq, mk, mv;
-    const int box_rows = page_size < XT_BN ? page_size : XT_BN;
-    if ((rc = map_queries(&mq, q, q_stride, H, tokens, G, per_tile)) != 0) return rc;
-    if ((rc = map_rows(&mk, k_cache, (uint64_t)cache_rows, (uint32_t)box_rows)) != 0) return rc;
-    if ((rc = map_rows(&mv, v_cache, (uint64_t)cache_rows, (uint32_t)box_rows)) != 0) return rc;
-    const CrossTc arg = {{q, k_cache, v_cache, out, block_table, lens, cu_tokens, spans, q_stride, max_pages, K, G, D, shift, scale}, error_flag, first_request, (int)pairs,
-                         (int)cache_rows};
-    return launch_kernel(attention_cross_tc_kernel, dim3((unsigned)(requests * pairs), K, chunks), dim3(XT_THREADS), XT_SMEM, s, chunks, mq, mk, mv, arg);
+    const int box_rows = c->page_size < XT_BN ? c->page_size : XT_BN;
+    if ((rc = map_queries(&mq, c->q, c->q_stride, c->H, c->tokens, G, per_tile)) != 0) return rc;
+    if ((rc = map_rows(&mk, c->k_cache, (uint64_t)cache_rows, (uint32_t)box_rows)) != 0) return rc;
+    if ((rc = map_rows(&mv, c->v_cache, (uint64_t)cache_rows, (uint32_t)box_rows)) != 0) return rc;
+    const CrossTc arg = {cross_args(c), c->error_flag, c->first, (int)pairs, (int)cache_rows};
+    return launch_kernel(attention_cross_tc_kernel, dim3((unsigned)(c->requests * pairs), c->K, c->chunks), dim3(XT_THREADS), XT_SMEM, s, c->chunks, mq, mk, mv, arg);
 }

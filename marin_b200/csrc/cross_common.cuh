@@ -21,6 +21,34 @@ struct CrossArgs {
     float scale;
 };
 
+// What a call hands over, in one piece (a caller in Python pays for every argument): requests first .. first + requests - 1 of a step of `tokens` tokens, none
+// with more than max_query of them or a source longer than `longest`; chunks: how many blocks of a cluster share their keys (where the caller decides that).
+struct CrossCall {
+    const void *q, *k_cache, *v_cache;
+    void* out;
+    const int *block_table, *lens, *cu_tokens, *spans;
+    int* error_flag;
+    long long q_stride, cache_pages;
+    float scale;
+    int dtype, max_pages, first, requests, max_query, tokens, chunks, longest, H, K, d, page_size;
+};
+static inline int page_shift_of(int page_size) {
+    for (int b = 0; b < 24; ++b)
+        if ((1 << b) == page_size) return b;
+    return -1;
+}
+static inline CrossArgs cross_args(const CrossCall* c) {
+    return {c->q, c->k_cache, c->v_cache, c->out, c->block_table, c->lens, c->cu_tokens, c->spans, c->q_stride, c->max_pages, c->K, c->H / c->K, c->d,
+            page_shift_of(c->page_size), c->scale};
+}
+// What every kernel asks of a call: sizes that fit, a power of two of positions a page.
+static inline bool cross_call_fits(const CrossCall* c) {
+    const int shift = page_shift_of(c->page_size);
+    return shift >= 0 && c->K > 0 && c->K <= 65535 && c->H > 0 && c->H % c->K == 0 && c->d > 0 && c->max_pages >= 0 && ((long long)c->max_pages << shift) <= 0x7fffff00LL &&
+           c->scale > 0.0f;
+}
+static inline bool chunks_fit(int chunks) { return chunks == 1 || chunks == 2 || chunks == 4 || chunks == 8; }
+
 // The positions token t of a request sees, cut to its source; (0, 0) where there are none.
 __device__ __forceinline__ int2 cross_range(const CrossArgs& a, int t, int len) {
     int lo = 0, hi = len;

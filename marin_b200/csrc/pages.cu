@@ -157,13 +157,21 @@ static bool overlap(const void* a, size_t na, const void* b, size_t nb) {
 // before, after [R], table [R, columns], free [free_size], count [1], left [2], cu [R + 1], req, pos, slots [room]: int32.  page_size: a power of two.
 // left[1]: 0; 1: the free list runs out of pages; 2: more new tokens than `room`; 3: a length is negative or needs more pages than a row of the table
 // has; 4: the free list cannot hold what is given back (or `count` is none of its lengths).  Where it is not 0 nothing is taken or given back.
-MB_API int mb_page_step(const int* before, const int* after, int* table, int* free, const int* count, int* left, int* cu, int* req, int* pos, int* slots,
-                        int R, int columns, int free_size, int page_size, int room, cudaStream_t s) {
+struct PageStepCall {              // (in one piece: a caller in Python pays for every argument)
+    const int *before, *after;
+    int *table, *free;
+    const int* count;
+    int *left, *cu, *req, *pos, *slots;
+    int R, columns, free_size, page_size, room;
+};
+
+MB_API int mb_page_step(const PageStepCall* c, cudaStream_t s) {
+    const int R = c->R, columns = c->columns, free_size = c->free_size, page_size = c->page_size, room = c->room;
     if (R <= 0 || R > PG_MAX_REQUESTS || columns <= 0 || (long long)R * columns >= PG_LIMIT || free_size < 0 || free_size >= (int)PG_LIMIT || room < 0 ||
         room >= (int)PG_LIMIT || page_size <= 0 || (page_size & (page_size - 1)) != 0)
         return MB_ERR_BAD_SIZE;
     // what every block reads must not be what another has written by then
-    const void* part[] = {before, after, count, table, free, left, cu, req, pos, slots};
+    const void* part[] = {c->before, c->after, c->count, c->table, c->free, c->left, c->cu, c->req, c->pos, c->slots};
     const size_t n[] = {(size_t)R, (size_t)R, 1, (size_t)R * columns, (size_t)free_size, 2, (size_t)R + 1, (size_t)room, (size_t)room, (size_t)room};
     for (int i = 0; i < 10; ++i)
         for (int j = i + 1; j < 10; ++j)
@@ -176,6 +184,6 @@ MB_API int mb_page_step(const int* before, const int* after, int* table, int* fr
     static LaunchSmem allowed;
     const int rc = allowed.allow(page_step_kernel, 3 * (PG_MAX_REQUESTS + 1) * sizeof(unsigned));
     if (rc != 0) return rc;
-    const PageStep p = {before, after, table, free, count, left, cu, req, pos, slots, R, columns, free_size, shift, room};
+    const PageStep p = {c->before, c->after, c->table, c->free, c->count, c->left, c->cu, c->req, c->pos, c->slots, R, columns, free_size, shift, room};
     return launch_kernel(page_step_kernel, dim3(blocks), dim3(threads), smem, s, 0, p);
 }

@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import struct
 import weakref
 from typing import Optional
 
@@ -2808,7 +2809,7 @@ def gla_jobs(dtype, d: int, dv: int, rank: int) -> dict:
 
 # ---- a decoder that reads an encoder's states: heads with positions of several axes, the states' pages, attention to them ----
 
-def _on_current_device(*tensors) -> int:
+def _on_current_device(what: str, *tensors) -> int:
     """The current device: launches go to its current stream, and tensors of another device (or of the host) are refused."""
     here = None
     for t in tensors:
@@ -2817,29 +2818,32 @@ def _on_current_device(*tensors) -> int:
             if here is None and d >= 0:
                 here = _current_device()
             if d != here:
-                raise KernelError(f"marin_b200 kernels run on tensors of the current CUDA device; there is no CPU path: got one on {t.device}")
+                raise KernelError(f"{what}: marin_b200 kernels run on tensors of the current CUDA device; there is no CPU path: got one on {t.device}")
     return here
 
 
-def _int32(what: str, *tensors) -> None:
+def _int32_on(what: str, here: Optional[int], tensors) -> int:
+    """The same for tensors that hold contiguous 32-bit whole numbers."""
     for t in tensors:
-        if t.dtype is not torch.int32 or not t.is_contiguous():
-            raise KernelError(f"{what}: expects contiguous int32 tensors, got {t.dtype}")
+        d = t.get_device()
+        if d != here or d < 0 or t.dtype is not torch.int32 or not t.is_contiguous():
+            if here is not None or d < 0 or d != _current_device() or t.dtype is not torch.int32 or not t.is_contiguous():
+                raise KernelError(f"{what}: expects contiguous int32 tensors on the current CUDA device, got {t.dtype} on {t.device}")
+            here = d
+    return here
 
 
-_entries: dict = {}
-_KINDS = {"p": _c_void_p, "i": _c_int, "l": ctypes.c_longlong, "f": _c_float}
+#: A call of a few microseconds is bound by the host, and ctypes takes a tenth of one for every argument: these entry points take theirs in one packed piece.
+_PAGE_STEP, _HEADS_AXES, _CROSS = (struct.Struct(f) for f in ("10P5i", "10P2qf10i", "9P2qf12i"))
+_packed_entries: dict = {}
 
 
-def _entry(lib, name: str, kinds: str):
-    """A library's function with its arguments' types said once (p: an address or None, i, l: whole numbers of 32 and 64 bits, f: a float): a call then takes plain
-    Python numbers, half a microsecond an argument less than wrapping each (calls of a few microseconds are bound by the host)."""
-    key = (lib._name, name)
-    fn = _entries.get(key)
+def _packed_entry(name: str, load):
+    fn = _packed_entries.get(name)
     if fn is None:
-        fn = getattr(lib, name)
-        fn.argtypes = [_KINDS[k] for k in kinds]
-        _entries[key] = fn
+        fn = getattr(load(), name.split(" ")[0])
+        fn.argtypes = [ctypes.c_char_p, _c_void_p]
+        _packed_entries[name] = fn
     return fn
 
 
@@ -2847,8 +2851,8 @@ def _stream_of(device: int):
     return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
 
-def _address(t: Optional[torch.Tensor]):
-    return t.data_ptr() if t is not None else None
+def _address(t: Optional[torch.Tensor]) -> int:
+    return t.data_ptr() if t is not None else 0
 
 
 def axis_sections(sections, spread: bool = False) -> list:
@@ -2876,42 +2880,49 @@ def qk_norm_axes_write(rows: torch.Tensor, q_out: Optional[torch.Tensor], q_weig
     ``inv_freq`` float32 ``[rotary_dim / 2]``; the angle in 64 bits); queries go to ``q_out`` ``[T, H * d]``, keys and values into the paged caches at ``slot_mapping``
     (negative: a padded token, nothing is stored).  ``rows`` ``[T, >= (H + 2 K) * d]`` may be columns of wider rows.  ``H = 0`` (``q_out`` None): an encoder's
     keys and values alone; ``write_kv=False``: queries alone.  ``axis_of`` is held to the axes there are, places past the caches store nothing."""
-    device = _on_current_device(rows, q_out, q_weight, k_weight, positions, axis_of, inv_freq, slot_mapping, k_cache, v_cache)
-    if rows.dim() != 2:
-        raise KernelError(f"qk_norm_axes_write: rows are [T, columns], got {tuple(rows.shape)}")
-    T = rows.shape[0]
+    device = _on_current_device("qk_norm_axes_write", rows, q_out, q_weight, k_weight, positions, axis_of, inv_freq, slot_mapping, k_cache, v_cache)
+    shape, dtype = rows.shape, rows.dtype
     wanted = (H + 2 * K if write_kv else H) * d
-    if rows.shape[1] < wanted or H < 0 or K < 0 or wanted <= 0 or (rows.shape[1] > 1 and rows.stride(1) != 1):
-        raise KernelError(f"qk_norm_axes_write: {tuple(rows.shape)} is not rows of {H} query and {K if write_kv else 0} key and value heads of {d}")
-    if H > 0 and (q_out is None or tuple(q_out.shape) != (T, H * d) or q_out.dtype != rows.dtype or not q_out.is_contiguous()):
-        raise KernelError(f"qk_norm_axes_write: q_out is a contiguous {rows.dtype} tensor [{T}, {H * d}]")
+    if len(shape) != 2 or shape[1] < wanted or H < 0 or K < 0 or wanted <= 0:
+        raise KernelError(f"qk_norm_axes_write: {tuple(shape)} is not rows of {H} query and {K if write_kv else 0} key and value heads of {d}")
+    T, (row_stride, column_stride) = shape[0], rows.stride()
+    if column_stride != 1:
+        raise KernelError("qk_norm_axes_write: a row's elements have to lie side by side")
+    if H > 0 and (q_out is None or q_out.shape != (T, H * d) or q_out.dtype is not dtype or not q_out.is_contiguous()):
+        raise KernelError(f"qk_norm_axes_write: q_out is a contiguous {dtype} tensor [{T}, {H * d}]")
     for w in (q_weight, k_weight):
-        if w is not None and (w.dtype != torch.float32 or w.numel() != d or not w.is_contiguous()):
+        if w is not None and (w.dtype is not torch.float32 or w.numel() != d or not w.is_contiguous()):
             raise KernelError(f"qk_norm_axes_write: norm weights are float32 [{d}]")
-    if inv_freq is not None:
+    axes = 0
+    if inv_freq is None:
+        rotary_dim = 0
+    else:
         if rotary_dim <= 0 or rotary_dim > d or rotary_dim % 2:
             raise KernelError(f"qk_norm_axes_write: rotary_dim {rotary_dim} must be even and within the head's {d}")
-        _int32("qk_norm_axes_write", positions, axis_of)
-        if (positions.dim() != 2 or positions.shape[1] != T or positions.shape[0] < 1 or axis_of.numel() != rotary_dim // 2 or inv_freq.numel() != rotary_dim // 2
-                or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous()):
+        _int32_on("qk_norm_axes_write", device, (positions, axis_of))
+        if (positions.dim() != 2 or positions.shape[1] != T or axis_of.numel() != rotary_dim // 2 or inv_freq.numel() != rotary_dim // 2
+                or inv_freq.dtype is not torch.float32 or not inv_freq.is_contiguous()):
             raise KernelError(f"qk_norm_axes_write: positions are [axes, {T}], axis_of and inv_freq [{rotary_dim // 2}]")
+        axes = positions.shape[0]
+        if axes < 1:
+            raise KernelError("qk_norm_axes_write: positions of one axis at least")
     page_size = cache_rows = 0
     if write_kv:
-        _int32("qk_norm_axes_write", slot_mapping)
-        if (k_cache.dtype != rows.dtype or v_cache.dtype != rows.dtype or k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1] != K or k_cache.shape[3] != d
+        _int32_on("qk_norm_axes_write", device, (slot_mapping,))
+        cache = k_cache.shape
+        if (k_cache.dtype is not dtype or v_cache.dtype is not dtype or len(cache) != 4 or cache != v_cache.shape or cache[1] != K or cache[3] != d
                 or not k_cache.is_contiguous() or not v_cache.is_contiguous() or slot_mapping.numel() != T):
-            raise KernelError(f"qk_norm_axes_write: caches are contiguous {rows.dtype} [pages, {K}, page_size, {d}] with a slot for each of {T} tokens")
-        page_size = k_cache.shape[2]
-        cache_rows = k_cache.shape[0] * page_size
+            raise KernelError(f"qk_norm_axes_write: caches are contiguous {dtype} [pages, {K}, page_size, {d}] with a slot for each of {T} tokens")
+        page_size = cache[2]
+        cache_rows = cache[0] * page_size
     if T == 0:
         return
     if launch_log is not None:
-        _cost(2 * T * wanted * rows.element_size() + (_size(positions) if inv_freq is not None else 0), 8.0 * T * wanted)
-    turns = inv_freq is not None
-    _check(_entry(_lib("mb_rope_axes"), "mb_heads_axes", "pilpppfpippiipppliiiiiip")(
-        rows.data_ptr(), _code(rows), rows.stride(0), _address(q_out), _address(q_weight), _address(k_weight), eps, _address(positions), positions.shape[0] if turns else 0,
-        _address(axis_of), _address(inv_freq), rotary_dim if turns else 0, int(interleaved), _address(slot_mapping), _address(k_cache), _address(v_cache), cache_rows, page_size,
-        T, H, K, d, int(write_kv), _stream_of(device)), "qk_norm_axes_write")
+        _cost(2 * T * wanted * rows.element_size() + 4 * axes * T, 8.0 * T * wanted)
+    _check(_packed_entry("mb_heads_axes", lambda: _lib("mb_rope_axes"))(_HEADS_AXES.pack(
+        rows.data_ptr(), _address(q_out), _address(q_weight), _address(k_weight), _address(positions), _address(axis_of), _address(inv_freq), _address(slot_mapping),
+        _address(k_cache), _address(v_cache), row_stride, cache_rows, eps, _code(rows), axes, rotary_dim, int(interleaved), page_size, T, H, K, d, int(write_kv)),
+        _stream_of(device)), "qk_norm_axes_write")
 
 
 #: most requests of one ``page_step`` (the running sums over them lie in a block's shared memory)
@@ -2929,21 +2940,20 @@ def page_step(before: torch.Tensor, after: torch.Tensor, table: torch.Tensor, fr
 
     All or nothing: where ``left[1]`` is 1 (the free list runs out), 2 (more new tokens than the buffers' room), 3 (a length is negative or longer than a row of the
     table) or 4 (``count`` or what is given back is more than ``free`` holds), no page moves, ``left[0]`` is ``count[0]`` and every token is a padded one."""
-    device = _on_current_device(before, after, table, free, count, left, cu_tokens, req_index, positions, slots)
-    _int32("page_step", before, after, table, free, count, left, cu_tokens, req_index, positions, slots)
-    R, room = before.numel(), slots.numel()
+    device = _int32_on("page_step", None, (before, after, table, free, count, left, cu_tokens, req_index, positions, slots))
+    R, room, shape = before.numel(), slots.numel(), table.shape
     if R < 1 or R > PAGE_STEP_REQUESTS:
         raise KernelError(f"page_step: 1 to {PAGE_STEP_REQUESTS} requests, got {R}")
-    if (after.numel() != R or table.dim() != 2 or table.shape[0] != R or table.shape[1] < 1 or count.numel() != 1 or left.numel() != 2 or cu_tokens.numel() != R + 1
+    if (after.numel() != R or len(shape) != 2 or shape[0] != R or shape[1] < 1 or count.numel() != 1 or left.numel() != 2 or cu_tokens.numel() != R + 1
             or req_index.numel() != room or positions.numel() != room):
         raise KernelError(f"page_step: after [{R}], table [{R}, columns], count [1], left [2], cu_tokens [{R + 1}] and buffers of one size are wanted")
     if page_size < 1 or page_size & (page_size - 1):
         raise KernelError(f"page_step: page_size {page_size} is no power of two")
     if launch_log is not None:
         _cost(4 * (2 * R + R + 1 + 3 * room))
-    _check(_entry(_lib("mb_pages"), "mb_page_step", "ppppppppppiiiiip")(
+    _check(_packed_entry("mb_page_step", lambda: _lib("mb_pages"))(_PAGE_STEP.pack(
         before.data_ptr(), after.data_ptr(), table.data_ptr(), free.data_ptr(), count.data_ptr(), left.data_ptr(), cu_tokens.data_ptr(), req_index.data_ptr(), positions.data_ptr(),
-        slots.data_ptr(), R, table.shape[1], free.numel(), page_size, room, _stream_of(device)), "page_step (tensors must not overlap)")
+        slots.data_ptr(), R, shape[1], free.numel(), page_size, room), _stream_of(device)), "page_step (tensors must not overlap)")
 
 
 class Source:
@@ -3009,48 +3019,43 @@ def attention_cross(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     takes ``num_requests``, ``num_decode`` (the first requests, one token each), ``max_query_len`` and ``cu_tokens``; rows of ``q`` ``[T, H * d]`` past the last request's
     are not read and those of ``out`` stay as they were.  ``q`` may be columns of wider rows."""
     table, lens, cu = source.block_table, source.lens, ctx.cu_tokens
-    device = _on_current_device(q, k_cache, v_cache, out, table, lens, cu, spans)
-    R, nd, dtype, shape, cache = ctx.num_requests, ctx.num_decode, q.dtype, q.shape, k_cache.shape
-    if H <= 0 or K <= 0 or H % K or len(shape) != 2 or shape[1] != H * d or out.shape != shape or out.dtype is not dtype or not out.is_contiguous() or (shape[1] > 1 and q.stride(1) != 1):
+    device = _on_current_device("attention_cross", q, k_cache, v_cache, out)
+    _int32_on("attention_cross", device, (table, lens, cu) if spans is None else (table, lens, cu, spans))
+    R, nd, dtype, shape, cache, columns = ctx.num_requests, ctx.num_decode, q.dtype, q.shape, k_cache.shape, table.shape
+    if H <= 0 or K <= 0 or H % K or len(shape) != 2 or shape[1] != H * d or out.shape != shape or out.dtype is not dtype or not out.is_contiguous():
         raise KernelError(f"attention_cross: queries and results are [T, {H * d}] of one dtype ({H} heads over {K} of {d}), got {tuple(shape)} and {tuple(out.shape)}")
     if (k_cache.dtype is not dtype or v_cache.dtype is not dtype or len(cache) != 4 or cache != v_cache.shape or cache[1] != K or cache[3] != d
             or not k_cache.is_contiguous() or not v_cache.is_contiguous()):
         raise KernelError(f"attention_cross: caches are contiguous {dtype} [pages, {K}, page_size, {d}]")
-    T, pages, page_size = shape[0], cache[0], cache[2]
+    T, pages, page_size, (stride, column_stride) = shape[0], cache[0], cache[2], q.stride()
+    if column_stride != 1:
+        raise KernelError("attention_cross: a query row's elements have to lie side by side")
     if page_size < 1 or page_size & (page_size - 1) or d > 256:
         raise KernelError(f"attention_cross: pages of a power of two of positions and heads of up to 256, got {page_size} and {d}")
-    _int32("attention_cross", table, lens, cu)
-    if table.dim() != 2 or table.shape[0] < R or lens.numel() < R or cu.numel() < R + 1 or not 0 <= nd <= R:
+    if len(columns) != 2 or columns[0] < R or lens.numel() < R or cu.numel() < R + 1 or not 0 <= nd <= R:
         raise KernelError(f"attention_cross: block_table [{R}, pages], lens [{R}] and cu_tokens [{R + 1}] are wanted")
-    if spans is not None:
-        _int32("attention_cross", spans)
-        if spans.dim() != 2 or spans.shape[0] != T or spans.shape[1] != 2:
-            raise KernelError(f"attention_cross: spans are [{T}, 2]")
+    if spans is not None and spans.shape != (T, 2):
+        raise KernelError(f"attention_cross: spans are [{T}, 2]")
     if not 0.0 < scale < float("inf"):
         raise KernelError(f"attention_cross: scale is a positive number, got {scale}")
     if T == 0 or R == 0:
         return
-    longest, most, columns, stride = max(0, int(source.longest)), ctx.max_query_len, table.shape[1], q.stride(0)
-    addresses = (q.data_ptr(), stride, k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr())
-    where = (table.data_ptr(), columns, lens.data_ptr(), cu.data_ptr(), _address(spans))
-    aligned = stride % 8 == 0 and (addresses[0] | addresses[2] | addresses[3] | addresses[4]) % 16 == 0
-    tc = aligned and cross_tc_supported(dtype, H, K, d, page_size) and 0 < pages * K * page_size < 0x7fffff00
-    single = aligned and cross_decode_supported(dtype, H, K, d, page_size)
-    stream, group = _stream_of(device), H // K
-    for first, n, most, which in ((0, nd, 1, "decode"), (nd, R - nd, most, "portions")):
+    longest, group = max(0, int(source.longest)), H // K
+    at = (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr())
+    aligned = stride % 8 == 0 and (at[0] | at[1] | at[2] | at[3]) % 16 == 0
+    where = (table.data_ptr(), lens.data_ptr(), cu.data_ptr(), _address(spans), _scratch_for(q.device).error.data_ptr(), stride, pages, scale, _code(q), columns[1])
+    stream = _stream_of(device)
+    for first, n, most, single in ((0, nd, 1, True), (nd, R - nd, ctx.max_query_len, False)):
         if n <= 0:
             continue
         if launch_log is not None:
-            rows, size = (n if which == "decode" else T - nd), q.element_size()
+            rows, size = (n if single else T - nd), q.element_size()
             _cost(size * (2 * rows * H * d + 2 * n * longest * K * d), 4.0 * rows * longest * H * d)
-        if single and most == 1:
-            _check(_entry(_cross_lib("decode", d), "mb_attention_cross_decode", "plppppipppiiiiiifp")(
-                *addresses, *where, first, n, cross_decode_chunks(n * K, longest), H, K, page_size, scale, stream), f"attention_cross ({which})")
-        elif tc:
+        if single and aligned and cross_decode_supported(dtype, H, K, d, page_size):
+            fn, chunks, what = _packed_entry(f"mb_attention_cross_decode {d}", lambda: _cross_lib("decode", d)), cross_decode_chunks(n * K, longest), "attention_cross (single tokens)"
+        elif aligned and cross_tc_supported(dtype, H, K, d, page_size) and 0 < pages * K * page_size < 0x7fffff00:
             pairs = -(-most // (2 * (128 // group)))
-            _check(_entry(_cross_lib("tc", d), "mb_attention_cross_tc", "plppppipppiiiiiiiilfpp")(
-                *addresses, *where, first, n, most, T, cross_chunks(min(n * pairs, n + T * group // 256) * K, longest), H, K, page_size, pages, scale,
-                _scratch_for(q.device).error.data_ptr(), stream), f"attention_cross ({which}, tensor cores)")
+            fn, chunks, what = _packed_entry(f"mb_attention_cross_tc {d}", lambda: _cross_lib("tc", d)), cross_chunks(min(n * pairs, n + T * group // 256) * K, longest), "attention_cross (tensor cores)"
         else:
-            _check(_entry(_lib("mb_attention_cross"), "mb_attention_cross", "plpppipipppiiiiiiiifp")(
-                *addresses, _code(q), *where, first, n, most, longest, H, K, d, page_size, scale, stream), f"attention_cross ({which})")
+            fn, chunks, what = _packed_entry("mb_attention_cross", lambda: _lib("mb_attention_cross")), 0, "attention_cross"
+        _check(fn(_CROSS.pack(*at, *where, first, n, most, T, chunks, longest, H, K, d, page_size), stream), what)
