@@ -20,6 +20,7 @@
 #define MB_LIB_ID 43
 #include "tc_common.cuh"
 #include "cross_common.cuh"
+#include "pair_math.cuh"
 
 #ifndef HEAD_DIM
 #error "compile with -DHEAD_DIM=<multiple of 16, at most 128>"
@@ -62,17 +63,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-__device__ __forceinline__ uint64_t pair_of(float a, float b) {
-    uint64_t v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
-    return v;
-}
-__device__ __forceinline__ void of_pair(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
 __device__ __forceinline__ float max_nan(float a, float b) {
     float d;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
@@ -97,12 +87,6 @@ __device__ __forceinline__ void exp2_pair_poly(uint64_t x, float& p0, float& p1)
     p0 = __int_as_float(__float_as_int(p0) + (__float_as_int(n0) << 23));
     p1 = __int_as_float(__float_as_int(p1) + (__float_as_int(n1) << 23));
 }
-__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-
 // 32 columns of this thread's lane; nothing of v may be used before tmem_ld_wait.
 __device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, float* v) {
     asm volatile(

@@ -11,8 +11,13 @@
 #define MB_LIB_ID 41
 #include "common.cuh"
 #include "launch.cuh"
+#include "mma_helpers.cuh"
+#include "pair_math.cuh"
 
-#define AX_FEW 296                 // tokens a block each: up to two blocks an SM
+#ifndef AX_STAGES
+#define AX_STAGES 3                // tokens whose rows are on their way
+#endif
+#define AX_SMS 148
 
 struct AxesRows {
     const void* rows;              // [T] rows `row_stride` elements apart: H query heads, K key heads, K value heads of d
@@ -30,11 +35,12 @@ struct AxesRows {
     int T, H, K, d, axes, half, interleaved, page_size, heads_total;
 };
 
-// cos and sin of token t's angle of pair f.
+// Sine and cosine of an angle given in turns.
+__device__ __forceinline__ void turn_of(double turns, float* sn, float* cs) { sincospif(2.0f * (float)(turns - rint(turns)), sn, cs); }
+// The same of token t's angle of pair f (1 / (2 pi) turns a radian).
 __device__ __forceinline__ void token_angle(const AxesRows& p, int t, int f, float* cs, float* sn) {
     const int axis = min(max(p.axis_of[f], 0), p.axes - 1);
-    const double turns = (double)p.positions[(size_t)axis * p.T + t] * (double)p.inv_freq[f] * 0.15915494309189533577;
-    sincospif(2.0f * (float)(turns - rint(turns)), sn, cs);
+    turn_of((double)p.positions[(size_t)axis * p.T + t] * ((double)p.inv_freq[f] * 0.15915494309189533577), sn, cs);
 }
 
 // Where head `head` of token t goes, or null.
@@ -46,126 +52,194 @@ __device__ __forceinline__ T* head_out(const AxesRows& p, int t, int head, int s
     return (T*)(head < p.H + p.K ? p.k_cache : p.v_cache) + (((size_t)(slot / p.page_size) * p.K + kh) * p.page_size + (size_t)(slot % p.page_size)) * p.d;
 }
 
+// 16 bytes of a head as pairs of float32, and back (rounded to nearest).
 template <typename T> struct Vec;
 template <> struct Vec<bf16> {
     static constexpr int N = 8;
-    static __device__ __forceinline__ void unpack(const uint4& raw, float* v) {
-        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
+    static __device__ __forceinline__ void unpack(const uint4& raw, uint64_t* v) {
+        const uint32_t r[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { const float2 f = __bfloat1622float2(h[i]); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
+        for (int i = 0; i < 4; ++i) v[i] = pair_of(__uint_as_float(r[i] << 16), __uint_as_float(r[i] & 0xffff0000u));
     }
-    static __device__ __forceinline__ uint4 pack(const float* v) {
-        uint4 raw;
-        __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&raw);
+    static __device__ __forceinline__ uint4 pack(const uint64_t* v) {
+        uint32_t r[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-        return raw;
+        for (int i = 0; i < 4; ++i) {
+            float x, y;
+            of_pair(v[i], x, y);
+            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r[i]) : "f"(y), "f"(x));
+        }
+        return make_uint4(r[0], r[1], r[2], r[3]);
     }
 };
 template <> struct Vec<float> {
     static constexpr int N = 4;
-    static __device__ __forceinline__ void unpack(const uint4& raw, float* v) {
-        v[0] = __uint_as_float(raw.x); v[1] = __uint_as_float(raw.y); v[2] = __uint_as_float(raw.z); v[3] = __uint_as_float(raw.w);
+    static __device__ __forceinline__ void unpack(const uint4& raw, uint64_t* v) {
+        v[0] = pair_of(__uint_as_float(raw.x), __uint_as_float(raw.y));
+        v[1] = pair_of(__uint_as_float(raw.z), __uint_as_float(raw.w));
     }
-    static __device__ __forceinline__ uint4 pack(const float* v) { return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])); }
+    static __device__ __forceinline__ uint4 pack(const uint64_t* v) {
+        float x, y, z, w;
+        of_pair(v[0], x, y);
+        of_pair(v[1], z, w);
+        return make_uint4(__float_as_uint(x), __float_as_uint(y), __float_as_uint(z), __float_as_uint(w));
+    }
 };
+// N floats (at 16 bytes) as pairs; the same of half as many.
+template <int N>
+__device__ __forceinline__ void load_pairs(const float* from, uint64_t* v) {
+    if (N == 2) { const float2 f = *reinterpret_cast<const float2*>(from); v[0] = pair_of(f.x, f.y); }
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+        const float4 f = reinterpret_cast<const float4*>(from)[i];
+        v[2 * i] = pair_of(f.x, f.y);
+        v[2 * i + 1] = pair_of(f.z, f.w);
+    }
+}
+// Pairs side by side: (x, y) by the angle of each.
+template <int N>
+__device__ __forceinline__ void turn_inside(uint64_t* v, const float* c, const float* s) {
+    uint64_t cc[N / 4 > 0 ? N / 4 : 1], ss[N / 4 > 0 ? N / 4 : 1];
+    load_pairs<N / 2>(c, cc);
+    load_pairs<N / 2>(s, ss);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        float x, y, ce[2], se[2];
+        of_pair(v[i], x, y);
+        of_pair(cc[i >> 1], ce[0], ce[1]);
+        of_pair(ss[i >> 1], se[0], se[1]);
+        v[i] = pair_of(x * ce[i & 1] - y * se[i & 1], y * ce[i & 1] + x * se[i & 1]);
+    }
+}
 
-// LPG lanes a head (a power of two, at least the head's `units`), two vectors a lane, TT tokens a block.  Heads, halves and rows in whole 16-byte vectors.
-template <typename T, int LPG, bool SIDE, int TT>
-__global__ void __launch_bounds__(512) heads_axes_kernel(AxesRows p, int units) {
+// LPG lanes a head (a power of two, at least the head's `units`), two vectors a lane.  Heads, halves and rows in whole 16-byte vectors.
+// A block (x) takes `per_block` tokens one after the other, of the heads that its threads reach (y): the rows of the next AX_STAGES tokens are on their way
+// (cp.async, every thread the vectors that it works on itself, so no barrier stands between), and the angles of the next `ng` tokens are worked out, one a
+// thread, before those at hand are used.  A thread's head is the same throughout: its weights stay in registers, its addresses move by a row.
+template <typename T, int LPG, bool SIDE>
+__global__ void __launch_bounds__(512, 2) heads_axes_kernel(AxesRows p, int units, int ng, int per_block) {
     constexpr int N = Vec<T>::N;
-    extern __shared__ __align__(16) float ax_tab[];                 // [TT][half] cosines, [TT][half] sines
-    const int t0 = blockIdx.x * TT, here = min(TT, p.T - t0), sub = threadIdx.x % LPG, group = threadIdx.x / LPG, groups = blockDim.x / LPG;
-    const int vecs = p.d / N, turned = 2 * p.half / N;              // vectors of a head; the first `turned` of them turn
+    extern __shared__ __align__(16) uint8_t ax_smem[];
+    const int threads = blockDim.x, tid = threadIdx.x, sub = tid % LPG, half = p.half;
+    uint4* ring = reinterpret_cast<uint4*>(ax_smem) + tid;          // [stage][2][threads]
+    float* angles = reinterpret_cast<float*>(ax_smem + (size_t)AX_STAGES * 2 * threads * 16);       // [2][ng][cosines, sines][half]
+    long long* places = reinterpret_cast<long long*>(angles + 4 * ng * half);               // [2][ng]: the token's first element in a cache, or -1
+    const int vecs = p.d / N, turned = 2 * half / N;                // vectors of a head; the first `turned` of them turn
     // this lane's two vectors: the rotation's partners, or, of what does not turn (or turns inside a vector), the first and second half
     int va, vb;
     if (SIDE) { va = sub; vb = sub + units; }
     else if (sub < turned / 2) { va = sub; vb = sub + turned / 2; }
     else { va = turned + (sub - turned / 2); vb = va + (units - turned / 2); }
-    const bool has_a = sub < units && va < vecs, has_b = sub < units && vb < vecs;
+    const int head = blockIdx.y * (threads / LPG) + tid / LPG;
+    const bool valid = head < p.heads_total, has_a = valid && sub < units && va < vecs, has_b = valid && sub < units && vb < vecs;
+    const bool is_q = head < p.H, is_k = !is_q && head < p.H + p.K;
+    const bool turns_a = (is_q || is_k) && half > 0 && (SIDE ? va < turned : sub < turned / 2), turns_b = (is_q || is_k) && half > 0 && (SIDE ? vb < turned : sub < turned / 2);
+    const int t0 = blockIdx.x * per_block, n = min(per_block, p.T - t0);
     PDL_ENTER();
     p.rows = pdl_fresh((const char*)p.rows); p.positions = pdl_fresh(p.positions); p.slots = pdl_fresh(p.slots);
-    const T* row = (const T*)p.rows + (size_t)t0 * p.row_stride;
-    float* cs = ax_tab;
-    float* sn = ax_tab + TT * p.half;
-    const bool turns = SIDE ? true : sub < turned / 2;
-    const int rounds = (p.heads_total + groups - 1) / groups;       // the same for all lanes of a warp: the shuffles need them all
-    for (int k = 0; k < rounds; ++k) {
-        const int head = group + k * groups;
-        const bool valid = head < p.heads_total;
-        uint4 ra[TT], rb[TT];
-#pragma unroll
-        for (int j = 0; j < TT; ++j) {
-            ra[j] = rb[j] = make_uint4(0, 0, 0, 0);
-            if (valid && j < here) {
-                const T* at = row + (size_t)j * p.row_stride + (size_t)head * p.d;
-                if (has_a) ra[j] = *reinterpret_cast<const uint4*>(at + va * N);
-                if (has_b) rb[j] = *reinterpret_cast<const uint4*>(at + vb * N);
-            }
+    const T* from = (const T*)p.rows + (size_t)t0 * p.row_stride + (size_t)head * p.d;
+    const T *from_a = from + va * N, *from_b = from + vb * N;
+    int asked = 0, ask_stage = 0;
+    auto fetch = [&]() {
+        if (asked < n) {
+            if (has_a) cp_async16(ring + ask_stage * 2 * threads, from_a);
+            if (has_b) cp_async16(ring + (ask_stage * 2 + 1) * threads, from_b);
+            from_a += p.row_stride; from_b += p.row_stride;
         }
-        if (k == 0 && p.half > 0) {                                 // (the rows are on their way)
-            for (int i = threadIdx.x; i < here * p.half; i += blockDim.x) {
-                const int j = i / p.half, f = i - j * p.half;
-                token_angle(p, t0 + j, f, &cs[i], &sn[i]);
-            }
-            __syncthreads();
+        ++asked;
+        ask_stage = ask_stage + 1 == AX_STAGES ? 0 : ask_stage + 1;
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < AX_STAGES; ++i) fetch();
+    // angles and places of the tokens first .. first + ng - 1, into buffer `buf`
+    const bool all_at_once = ng * half <= threads, one_each = all_at_once && tid < ng * half;
+    const int my_token = half > 0 ? tid / half : 0, my_pair = half > 0 ? tid % half : 0;
+    const int my_axis = one_each ? min(max(p.axis_of[my_pair], 0), p.axes - 1) : 0;
+    const double my_freq = one_each ? (double)p.inv_freq[my_pair] * 0.15915494309189533577 : 0.0;
+    const int* my_positions = p.positions + (size_t)my_axis * p.T + t0 + my_token;
+    auto position_of = [&](int first) { return one_each && first + my_token < n ? my_positions[first] : 0; };
+    auto prepare = [&](int first, int buf, int position) {
+        if (first >= n) return;
+        float* cs = angles + buf * 2 * ng * half;
+        if (all_at_once) {
+            if (one_each) turn_of((double)position * my_freq, &cs[(2 * my_token + 1) * half + my_pair], &cs[2 * my_token * half + my_pair]);
+        } else {
+            for (int i = tid; i < ng * half; i += threads)
+                if (first + i / half < n) token_angle(p, t0 + first + i / half, i % half, &cs[2 * (i / half) * half + i % half], &cs[(2 * (i / half) + 1) * half + i % half]);
         }
-        const float* w = head < p.H ? p.q_w : (head < p.H + p.K ? p.k_w : nullptr);
+        if (tid < ng) {
+            const int slot = p.heads_total > p.H && first + tid < n ? p.slots[t0 + first + tid] : -1;
+            places[buf * ng + tid] = slot >= 0 && slot < p.cache_rows ? ((long long)(slot / p.page_size) * p.K * p.page_size + slot % p.page_size) * p.d : -1;
+        }
+    };
+    const float* w = is_q ? p.q_w : (is_k ? p.k_w : nullptr);
+    const bool any_norm = p.q_w != nullptr || p.k_w != nullptr;
+    const float inv_d = 1.0f / (float)p.d;
+    uint64_t wa[N / 2], wb[N / 2];
+    if (w != nullptr) {
+        if (has_a) load_pairs<N>(w + va * N, wa);
+        if (has_b) load_pairs<N>(w + vb * N, wb);
+    }
+    // where this thread's vectors go: a row of q_out a token, or from the token's place in a cache on
+    T* to = is_q ? (T*)p.q_out + ((size_t)t0 * p.H + head) * p.d : (T*)(is_k ? p.k_cache : p.v_cache) + (size_t)(head - p.H - (is_k ? 0 : p.K)) * p.page_size * p.d;
+    prepare(0, 0, position_of(0));
+    int position = position_of(ng), stage = 0;
+    for (int first = 0, buf = 0; first < n; first += ng, buf ^= 1) {
+        __syncthreads();                                            // (this buffer's angles are there, and nobody reads the other's)
+        prepare(first + ng, buf ^ 1, position);
+        position = position_of(first + 2 * ng);
+        const float* cs = angles + buf * 2 * ng * half;
+        const int last = min(ng, n - first);
+        for (int j = 0; j < last; ++j, cs += 2 * half) {
+            cp_async_wait<AX_STAGES - 1>();
+            uint64_t a[N / 2], b[N / 2];
+            Vec<T>::unpack(has_a ? ring[stage * 2 * threads] : make_uint4(0, 0, 0, 0), a);
+            Vec<T>::unpack(has_b ? ring[(stage * 2 + 1) * threads] : make_uint4(0, 0, 0, 0), b);
+            stage = stage + 1 == AX_STAGES ? 0 : stage + 1;
+            fetch();
+            if (any_norm) {
+                uint64_t sq = mul_pair(a[0], a[0]), sr = mul_pair(b[0], b[0]);
 #pragma unroll
-        for (int j = 0; j < TT; ++j) {
-            if (j >= here) break;
-            float a[N], b[N];
-            Vec<T>::unpack(ra[j], a);
-            Vec<T>::unpack(rb[j], b);
-            if (p.q_w != nullptr || p.k_w != nullptr) {
-                float ss = 0.0f;
-#pragma unroll
-                for (int e = 0; e < N; ++e) ss += a[e] * a[e] + b[e] * b[e];
+                for (int e = 1; e < N / 2; ++e) { sq = fma_pair(a[e], a[e], sq); sr = fma_pair(b[e], b[e], sr); }
+                float s0, s1;
+                of_pair(add_pair(sq, sr), s0, s1);
+                float ss = s0 + s1;
 #pragma unroll
                 for (int o = LPG / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
                 if (w != nullptr) {
-                    const float scale = 1.0f / sqrtf(ss / (float)p.d + p.eps);
-                    if (has_a) {
-#pragma unroll
-                        for (int e = 0; e < N; ++e) a[e] = a[e] * scale * w[va * N + e];
-                    }
-                    if (has_b) {
-#pragma unroll
-                        for (int e = 0; e < N; ++e) b[e] = b[e] * scale * w[vb * N + e];
-                    }
-                }
-            }
-            if (head < p.H + p.K && p.half > 0) {
-                const float *c = cs + j * p.half, *s = sn + j * p.half;
-                if (SIDE) {
+                    const float scale = rsqrtf(fmaf(ss, inv_d, p.eps));
+                    const uint64_t scales = pair_of(scale, scale);
 #pragma unroll
                     for (int e = 0; e < N / 2; ++e) {
-                        if (va < turned) {
-                            const float x = a[2 * e], y = a[2 * e + 1], ce = c[va * (N / 2) + e], se = s[va * (N / 2) + e];
-                            a[2 * e] = x * ce - y * se; a[2 * e + 1] = y * ce + x * se;
-                        }
-                        if (vb < turned) {
-                            const float x = b[2 * e], y = b[2 * e + 1], ce = c[vb * (N / 2) + e], se = s[vb * (N / 2) + e];
-                            b[2 * e] = x * ce - y * se; b[2 * e + 1] = y * ce + x * se;
-                        }
+                        a[e] = mul_pair(mul_pair(a[e], scales), wa[e]);
+                        b[e] = mul_pair(mul_pair(b[e], scales), wb[e]);
                     }
-                } else if (turns) {
+                }
+            }
+            if (SIDE) {
+                if (turns_a) turn_inside<N>(a, cs + va * (N / 2), cs + half + va * (N / 2));
+                if (turns_b) turn_inside<N>(b, cs + vb * (N / 2), cs + half + vb * (N / 2));
+            } else if (turns_a) {
+                uint64_t cc[N / 2], ss[N / 2];
+                load_pairs<N>(cs + sub * N, cc);
+                load_pairs<N>(cs + half + sub * N, ss);
 #pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        const float x = a[e], y = b[e], ce = c[sub * N + e], se = s[sub * N + e];
-                        a[e] = x * ce - y * se; b[e] = y * ce + x * se;
-                    }
+                for (int e = 0; e < N / 2; ++e) {
+                    const uint64_t x = a[e], y = b[e], minus = ss[e] ^ 0x8000000080000000ull;
+                    a[e] = fma_pair(x, cc[e], mul_pair(y, minus));
+                    b[e] = fma_pair(y, cc[e], mul_pair(x, ss[e]));
                 }
             }
-            if (valid) {
-                T* dst = head_out<T>(p, t0 + j, head, head < p.H ? 0 : p.slots[t0 + j]);
-                if (dst != nullptr) {
-                    if (has_a) *reinterpret_cast<uint4*>(dst + va * N) = Vec<T>::pack(a);
-                    if (has_b) *reinterpret_cast<uint4*>(dst + vb * N) = Vec<T>::pack(b);
-                }
+            const long long place = is_q ? 0 : places[buf * ng + j];
+            if (place >= 0) {
+                if (has_a) *reinterpret_cast<uint4*>(to + place + va * N) = Vec<T>::pack(a);
+                if (has_b) *reinterpret_cast<uint4*>(to + place + vb * N) = Vec<T>::pack(b);
             }
+            if (is_q) to += (size_t)p.H * p.d;
         }
     }
+    cp_async_wait<0>();
 }
 
 // Any head size, rotary width and alignment: a warp takes a head through shared memory.
@@ -189,7 +263,7 @@ __global__ void __launch_bounds__(128) heads_axes_any_kernel(AxesRows p) {
         for (int i = lane; i < p.d; i += 32) { const float v = to_f32(src[i]); buf[i] = v; ss += v * v; }
         const float* w = head < p.H ? p.q_w : (head < p.H + p.K ? p.k_w : nullptr);
         if (w != nullptr) {
-            const float scale = 1.0f / sqrtf(warp_sum(ss) / (float)p.d + p.eps);
+            const float scale = rsqrtf(warp_sum(ss) / (float)p.d + p.eps);
             for (int i = lane; i < p.d; i += 32) buf[i] = buf[i] * scale * w[i];
         }
         __syncwarp();
@@ -207,30 +281,37 @@ __global__ void __launch_bounds__(128) heads_axes_any_kernel(AxesRows p) {
     }
 }
 
+#define AX_SMEM_MOST (100 * 1024)
+template <typename T, int LPG, bool SIDE>
+static int ax_launch(dim3 grid, int threads, size_t smem, cudaStream_t s, const AxesRows& p, int units, int ng, int per_block) {
+    static LaunchSmem allowed;
+    const int rc = allowed.allow(heads_axes_kernel<T, LPG, SIDE>, AX_SMEM_MOST);
+    if (rc != 0) return rc;
+    return launch_kernel(heads_axes_kernel<T, LPG, SIDE>, grid, dim3(threads), smem, s, 0, p, units, ng, per_block);
+}
+
 template <typename T>
 static int launch_axes(const AxesRows& p, cudaStream_t s) {
     constexpr int N = Vec<T>::N;
     const uintptr_t all = (uintptr_t)p.rows | (uintptr_t)p.q_out | (uintptr_t)p.k_cache | (uintptr_t)p.v_cache;
-    const bool whole = p.d % N == 0 && (all & 15) == 0 && p.row_stride % N == 0 && (p.interleaved ? (2 * p.half) % N == 0 : p.half % N == 0);
+    const bool whole = p.d % N == 0 && ((all | (uintptr_t)p.q_w | (uintptr_t)p.k_w) & 15) == 0 && p.row_stride % N == 0 && (p.interleaved ? (2 * p.half) % N == 0 : p.half % N == 0);
     const int vecs = p.d / N, turned = 2 * p.half / N;
     const int units = p.interleaved ? (vecs + 1) / 2 : turned / 2 + (vecs - turned + 1) / 2;
-    if (whole && units <= 32) {
+    if (whole && units <= 32 && p.half <= 1024) {
         int lpg = 4;
         while (lpg < units) lpg <<= 1;
         const int threads = min(512, (p.heads_total * lpg + 31) / 32 * 32);
-        // many tokens: four a block, so that enough rows are on their way (8,007 tokens of 48 heads of 128: XX us, one a block 73); few: one, to have more blocks
-        const int tt = p.T >= 4 * AX_FEW ? 4 : 1;
-        const size_t smem = (size_t)max(1, 2 * tt * p.half) * sizeof(float);
-        const dim3 grid((p.T + tt - 1) / tt);
-#define AX_PICK(L, S) (tt == 4 ? launch_kernel(heads_axes_kernel<T, L, S, 4>, grid, dim3(threads), smem, s, 0, p, units) \
-                               : launch_kernel(heads_axes_kernel<T, L, S, 1>, grid, dim3(threads), smem, s, 0, p, units))
-#define AX_LAUNCH(L) (p.interleaved ? AX_PICK(L, true) : AX_PICK(L, false))
+        // Up to two blocks an SM, equal runs of tokens each; angles for as many tokens at once as a block has threads.
+        const int reach = threads / lpg, parts = (p.heads_total + reach - 1) / reach, blocks = max(1, 2 * AX_SMS / parts);
+        const int per_block = (p.T + blocks - 1) / blocks, ng = max(1, min(p.half > 0 ? threads / p.half : 8, per_block));
+        const size_t smem = (size_t)AX_STAGES * 2 * threads * 16 + (size_t)4 * ng * p.half * sizeof(float) + (size_t)2 * ng * sizeof(long long);
+        const dim3 grid((p.T + per_block - 1) / per_block, parts);
+#define AX_LAUNCH(L) (p.interleaved ? ax_launch<T, L, true>(grid, threads, smem, s, p, units, ng, per_block) : ax_launch<T, L, false>(grid, threads, smem, s, p, units, ng, per_block))
         if (lpg == 4) return AX_LAUNCH(4);
         if (lpg == 8) return AX_LAUNCH(8);
         if (lpg == 16) return AX_LAUNCH(16);
         return AX_LAUNCH(32);
 #undef AX_LAUNCH
-#undef AX_PICK
     }
     const size_t smem = (size_t)(4 * p.d + 2 * p.half) * sizeof(float);
     if (smem > 48 * 1024) return MB_ERR_BAD_SIZE;
