@@ -4,7 +4,7 @@
 // Every key and value of a request is read once for all heads of its kv head, so the bytes bound it.  A cluster of up to eight blocks takes one request and kv
 // head, each block an equal run of the positions (requests of a batch have sources of all lengths: shares by length keep the blocks of a cluster equal, where runs
 // of a fixed length leave most blocks of short ones idle); its four warps take stages of 16 positions in turn, each through a ring of its own (cp.async into padded
-// rows, three stages on their way a warp: 96 KB an SM's block), no barrier of the block in the loop.  The query heads are rows 0..7 of mma.sync.m16n8k16:
+// rows, two stages on their way a warp), no barrier of the block in the loop.  The query heads are rows 0..7 of mma.sync.m16n8k16:
 //   S = Q K^T   rows 8..15 of Q are zeros;
 //   O = P V     rows 0..7 hold a weight rounded to bfloat16, rows 8..15 what the rounding took off, rounded in turn: O's rows r and r + 8 add up to the weights'
 //               product at 16 bits of a weight, for no more products.
@@ -21,10 +21,12 @@
 static_assert(HEAD_DIM % 16 == 0 && HEAD_DIM >= 16 && HEAD_DIM <= 128, "heads in steps of 16 up to 128");
 
 #define D HEAD_DIM
+#ifndef XD_WARPS
 #define XD_WARPS 4
+#endif
 #define XD_KEYS 16                               // positions of a stage
 #ifndef XD_STAGES
-#define XD_STAGES 3
+#define XD_STAGES 2
 #endif
 #define XD_LD (D + 8)                            // elements of a padded row: ldmatrix without bank conflicts
 #define XD_STAGE_BYTES (2 * XD_KEYS * XD_LD * 2)
@@ -59,18 +61,6 @@ __global__ void __launch_bounds__(XD_WARPS * 32) attention_cross_decode_kernel(C
     const int share = (stages + cluster - 1) / cluster, mine0 = stage0 + rank * share, mine_n = max(0, min(share, stages - rank * share));
     const int steps = mine_n > warp ? (mine_n - warp + XD_WARPS - 1) / XD_WARPS : 0;
 
-    // the query rows straight into the MMA's A fragments: lane l holds row l / 4, columns 2 (l % 4) + {0, 1} and + 8 of every 16
-    uint32_t qa[D / 16][4];
-    {
-        const int row = lane >> 2;
-        const bf16* q = (const bf16*)a.q + (size_t)t * a.q_stride + (size_t)(kh * G + (row < G ? row : 0)) * D + 2 * (lane & 3);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-            qa[kk][0] = row < G ? *reinterpret_cast<const uint32_t*>(q + kk * 16) : 0u;
-            qa[kk][2] = row < G ? *reinterpret_cast<const uint32_t*>(q + kk * 16 + 8) : 0u;
-            qa[kk][1] = qa[kk][3] = 0u;
-        }
-    }
     uint8_t* ring = xd_smem + (size_t)warp * XD_RING;
     const size_t head_rows = (size_t)kh << a.page_shift, page_rows = (size_t)a.K << a.page_shift;
     // page of step i, for the 32 steps around: a lane a step
@@ -100,6 +90,18 @@ __global__ void __launch_bounds__(XD_WARPS * 32) attention_cross_decode_kernel(C
 #pragma unroll
     for (int i = 0; i < XD_STAGES; ++i) issue(i);
 
+    // the query rows straight into the MMA's A fragments: lane l holds row l / 4, columns 2 (l % 4) + {0, 1} and + 8 of every 16
+    uint32_t qa[D / 16][4];
+    {
+        const int row = lane >> 2;
+        const bf16* q = (const bf16*)a.q + (size_t)t * a.q_stride + (size_t)(kh * G + (row < G ? row : 0)) * D + 2 * (lane & 3);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+            qa[kk][0] = row < G ? *reinterpret_cast<const uint32_t*>(q + kk * 16) : 0u;
+            qa[kk][2] = row < G ? *reinterpret_cast<const uint32_t*>(q + kk * 16 + 8) : 0u;
+            qa[kk][1] = qa[kk][3] = 0u;
+        }
+    }
     const float sl2 = a.scale * 1.4426950408889634f;
     float m = -INFINITY, l = 0.0f;                                  // of this lane's row (query head lane / 4)
     float o[D / 8][4];                                              // [0], [1]: row lane / 4; [2], [3]: what the rounded weights left

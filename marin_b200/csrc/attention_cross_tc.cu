@@ -417,56 +417,86 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
         if (!(l_run < 1.0e30f)) l_run = __int_as_float(0x7fc00000);
         if (ok && steps > 0) ok = warp_wait(&o_done[tile * 2 + ((steps - 1) & 1)], ((steps - 1) >> 1) & 1, abort, error_flag, 47);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (cluster == 1 && two) {
-            bf16* dst = (bf16*)a.out + ((size_t)(tok0 + my_tok) * a.K * G + my_head) * D;
-            const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
-            bool odd = false;
-            if (ok) {
+        const int others = two ? nblk : (nblk + tile) >> 1;         // blocks of the other half
+        float* sO = (float*)smem + (size_t)tid * XT_OLD;
+        if (cluster > 1 || !two) {
+            // the tiles' memory is about to be written over: once every product of both halves is done
+            if (ok && others > 0) ok = warp_wait(&o_done[(1 - tile) * 2 + ((others - 1) & 1)], ((others - 1) >> 1) & 1, abort, error_flag, 47);
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+        }
+        // 16 columns of this row, or zeros where it had no block
+        auto load_o = [&](int c, float* o) {
+            if (steps > 0) {
+                tmem_ld16(o_col + c * 16, o);
+            } else {
 #pragma unroll
-                for (int c = 0; c < D / 16; ++c) {
-                    float o[16];
-                    if (steps > 0) tmem_ld16(o_col + c * 16, o);
-                    if (mine) {
-                        uint32_t w[8];
+                for (int j = 0; j < 16; ++j) o[j] = 0.0f;
+            }
+        };
+        float mine_f = 1.0f, other_f = 0.0f;                        // what this half's and B's partial results are multiplied by
+        if (!two) {
+            if (tile == 1) {
+                s_m[tid] = m_used; s_l[tid] = l_run;
+                if (ok) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float x = range.y > range.x ? o[2 * j] * inv : 0.0f, y = range.y > range.x ? o[2 * j + 1] * inv : 0.0f;
-                            odd |= !(fabsf(x) <= 3.0e38f) || !(fabsf(y) <= 3.0e38f);
-                            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[j]) : "f"(y), "f"(x));
-                        }
-                        reinterpret_cast<uint4*>(dst)[c * 2] = make_uint4(w[0], w[1], w[2], w[3]);
-                        reinterpret_cast<uint4*>(dst)[c * 2 + 1] = make_uint4(w[4], w[5], w[6], w[7]);
-                    }
-                }
-                if (a.spans != nullptr) {
-                    unsigned which = __ballot_sync(0xffffffffu, odd);
-                    for (; which != 0; which &= which - 1) {
-                        const int src = __ffs(which) - 1;
-                        const int tok = __shfl_sync(0xffffffffu, my_tok, src), head = __shfl_sync(0xffffffffu, my_head, src);
-                        const int2 rg = make_int2(__shfl_sync(0xffffffffu, range.x, src), __shfl_sync(0xffffffffu, range.y, src));
-                        __syncwarp();
-                        cross_row_alone<bf16>(arg.a, tok0 + tok, head, r, rg);
+                    for (int c = 0; c < D / 16; ++c) {
+                        float o[16];
+                        load_o(c, o);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(sO + c * 16 + 4 * j) = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
                     }
                 }
             }
-        } else {
-            // partial results into the tiles' memory, once every product of both halves is done
-            const int others = two ? nblk : (nblk + tile) >> 1;
-            if (ok && others > 0) ok = warp_wait(&o_done[(1 - tile) * 2 + ((others - 1) & 1)], ((others - 1) >> 1) & 1, abort, error_flag, 47);
             asm volatile("bar.sync 1, 256;" ::: "memory");
-            float* sO = (float*)smem + (size_t)tid * XT_OLD;
-            s_m[tid] = m_used; s_l[tid] = l_run;
-            if (ok) {
+            if (tile == 0) {
+                const float m_b = s_m[tid + XT_BM], top = fmaxf(m_used, m_b), base = top == -INFINITY ? 0.0f : top;
+                mine_f = xt_exp2(m_used - base); other_f = xt_exp2(m_b - base);
+                l_run = fmaf(mine_f, l_run, other_f * s_l[tid + XT_BM]);
+                m_used = top;
+            }
+        }
+        if (ok && (two || tile == 0)) {
+            bf16* dst = (bf16*)a.out + ((size_t)(tok0 + my_tok) * a.K * G + my_head) * D;
+            const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
+            const bool sees = range.y > range.x;
+            bool odd = false;
 #pragma unroll
-                for (int c = 0; c < D / 16; ++c) {
-                    float o[16];
-                    if (steps > 0) tmem_ld16(o_col + c * 16, o);
-                    else {
+            for (int c = 0; c < D / 16; ++c) {
+                float o[16];
+                load_o(c, o);
+                if (!two) {
+                    const float4* b = reinterpret_cast<const float4*>(sO + XT_BM * XT_OLD + c * 16);
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) o[j] = 0.0f;
+                    for (int j = 0; j < 4; ++j) {
+                        const float4 f = b[j];
+                        o[4 * j] = fmaf(mine_f, o[4 * j], other_f * f.x); o[4 * j + 1] = fmaf(mine_f, o[4 * j + 1], other_f * f.y);
+                        o[4 * j + 2] = fmaf(mine_f, o[4 * j + 2], other_f * f.z); o[4 * j + 3] = fmaf(mine_f, o[4 * j + 3], other_f * f.w);
                     }
+                }
+                if (cluster > 1) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(sO + c * 16 + 4 * j) = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                } else if (mine) {
+                    uint32_t w[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float x = sees ? o[2 * j] * inv : 0.0f, y = sees ? o[2 * j + 1] * inv : 0.0f;
+                        odd |= !(fabsf(x) <= 3.0e38f) || !(fabsf(y) <= 3.0e38f);
+                        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[j]) : "f"(y), "f"(x));
+                    }
+                    reinterpret_cast<uint4*>(dst)[c * 2] = make_uint4(w[0], w[1], w[2], w[3]);
+                    reinterpret_cast<uint4*>(dst)[c * 2 + 1] = make_uint4(w[4], w[5], w[6], w[7]);
+                }
+            }
+            if (cluster > 1) { s_m[tid] = m_used; s_l[tid] = l_run; }
+            if (a.spans != nullptr && cluster == 1) {
+                unsigned which = __ballot_sync(0xffffffffu, odd);
+                for (; which != 0; which &= which - 1) {
+                    const int src = __ffs(which) - 1;
+                    const int tok = __shfl_sync(0xffffffffu, my_tok, src), head = __shfl_sync(0xffffffffu, my_head, src);
+                    const int2 rg = make_int2(__shfl_sync(0xffffffffu, range.x, src), __shfl_sync(0xffffffffu, range.y, src));
+                    __syncwarp();
+                    cross_row_alone<bf16>(arg.a, tok0 + tok, head, r, rg);
                 }
             }
         }
@@ -475,42 +505,48 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (warp == 0) { __syncwarp(); tmem_free<false>(tmem_base, XT_TMEM); }
-    if (cluster > 1 || !two) {
-        if (cluster > 1) cross_cluster_sync();
-        // block `rank` finishes rows rank, rank + cluster, ...: a warp a row, the partial results in the order of ranks, and of A and B where both have the row
-        const int parts = two ? 1 : 2, rows = two ? 2 * XT_BM : XT_BM;
-        auto peer = [&](const float* at, int c) { return cluster > 1 ? cross_peer(smem_u32(at), c) : *at; };
+    if (cluster > 1) {
+        cross_cluster_sync();
+        // block `rank` finishes rows rank, rank + cluster, ...: a warp a row, the partial results in rank order (all asked for before the first is used)
         const float* sO = (const float*)smem;
-        for (int done = rank + warp * cluster; done < rows; done += (XT_THREADS / 32) * cluster) {
+        for (int done = rank + warp * cluster; done < (two ? 2 * XT_BM : XT_BM); done += (XT_THREADS / 32) * cluster) {
             const int in = done & (XT_BM - 1), tok = (done / XT_BM) * per_tile + in / G, head = kh * G + in % G;
             if (in >= per_tile * G || tok >= left) continue;
-            float top = -INFINITY, sum = 0.0f, v[(D + 31) / 32];
-            for (int c = 0; c < cluster; ++c)
-                for (int h = 0; h < parts; ++h) top = fmaxf(top, peer(&s_m[done + h * XT_BM], c));
+            constexpr int PIECES = (D + 31) / 32;
+            float w[XT_MAX_CLUSTER], u[XT_MAX_CLUSTER], part[XT_MAX_CLUSTER][PIECES], top = -INFINITY, sum = 0.0f, v[PIECES];
+#pragma unroll
+            for (int c = 0; c < XT_MAX_CLUSTER; ++c) {
+                const int from = c < cluster ? c : rank;
+                w[c] = cross_peer(smem_u32(&s_m[done]), from);
+                u[c] = cross_peer(smem_u32(&s_l[done]), from);
+#pragma unroll
+                for (int x = 0; x < PIECES; ++x) part[c][x] = cross_peer(smem_u32(sO + (size_t)done * XT_OLD + min(x * 32 + lane, D - 1)), from);
+            }
+#pragma unroll
+            for (int c = 0; c < XT_MAX_CLUSTER; ++c) top = fmaxf(top, w[c]);
             const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-            for (int x = 0; x < (D + 31) / 32; ++x) v[x] = 0.0f;
-            for (int c = 0; c < cluster; ++c)
-                for (int h = 0; h < parts; ++h) {
-                    const int at = done + h * XT_BM;
-                    const float w = xt_exp2(peer(&s_m[at], c) - base);
-                    sum = fmaf(w, peer(&s_l[at], c), sum);
+            for (int x = 0; x < PIECES; ++x) v[x] = 0.0f;
 #pragma unroll
-                    for (int x = 0; x < (D + 31) / 32; ++x)
-                        if (x * 32 + lane < D) v[x] = fmaf(w, peer(sO + (size_t)at * XT_OLD + x * 32 + lane, c), v[x]);
-                }
+            for (int c = 0; c < XT_MAX_CLUSTER; ++c) {
+                if (c >= cluster) continue;
+                const float f = xt_exp2(w[c] - base);
+                sum = fmaf(f, u[c], sum);
+#pragma unroll
+                for (int x = 0; x < PIECES; ++x) v[x] = fmaf(f, part[c][x], v[x]);
+            }
             const int2 rg = s_range[done];
             bf16* dst = (bf16*)a.out + ((size_t)(tok0 + tok) * a.K * G + head) * D;
             bool odd = false;
 #pragma unroll
-            for (int x = 0; x < (D + 31) / 32; ++x) {
+            for (int x = 0; x < PIECES; ++x) {
                 const float out = rg.y > rg.x && sum != 0.0f ? v[x] / sum : 0.0f;
                 odd |= !(fabsf(out) <= 3.0e38f);
                 if (x * 32 + lane < D) dst[x * 32 + lane] = __float2bfloat16_rn(out);
             }
             if (a.spans != nullptr && __any_sync(0xffffffffu, odd)) { __syncwarp(); cross_row_alone<bf16>(arg.a, tok0 + tok, head, r, rg); }
         }
-        if (cluster > 1) cross_cluster_sync();                      // (a block's shared memory is read until here)
+        cross_cluster_sync();                                       // (a block's shared memory is read until here)
     }
 }
 
