@@ -36,13 +36,27 @@ static_assert(HEAD_DIM % 16 == 0 && HEAD_DIM >= 16 && HEAD_DIM <= 128, "heads in
 #define XT_STAGES 4                             // blocks of keys, and of values, on their way
 #define XT_OLD (D + 4)                           // floats between rows of O for the cluster
 #define XT_BARS 512
+// 16-byte piece c of row r of a tile's results in shared memory: rows of whole 128 bytes swizzled, others a piece apart, so that neither a thread's row nor a
+// row across threads meets a bank twice
+#if HEAD_DIM % 64 == 0
+#define XT_STAGED(r, c) ((r) * (D / 8) + ((c) ^ ((r) & 7)))
+#else
+#define XT_STAGED(r, c) ((r) * (D / 8 + 1) + (c))
+#endif
 #define XT_SMEM (2 * XT_TILE + 2 * XT_STAGES * XT_KV + XT_BARS)
 static_assert(2 * XT_BM * XT_OLD * 4 <= 2 * XT_TILE + 2 * XT_STAGES * XT_KV, "partial results fit the tiles' memory");
-static_assert(XT_SMEM <= 232448 - 4608, "static shared memory is beside it");
+static_assert(D % 64 == 0 || XT_BM * (D * 2 + 16) <= XT_TILE, "a tile's results fit its queries' memory");
+static_assert(XT_BM * (D % 64 == 0 ? D * 2 : D * 2 + 16) <= XT_BM * XT_OLD * 4, "and lie ahead of B's partial results");
+static_assert(XT_SMEM <= 232448 - 6144, "static shared memory is beside it");
 #define XT_TMEM 512                              // two S buffers of A, of B (64 columns each), O of A, O of B (128)
 #define XT_O_COL 256
 #define XT_THREADS 384
 #define XT_MAX_CLUSTER 8
+// cycles: a block's way in and out, a cluster's meeting, 64 keys of two tiles, of one (see choose_chunks)
+#define XT_COST_BLOCK 9000
+#define XT_COST_CLUSTER 4000
+#define XT_COST_KEYS 1400
+#define XT_COST_SOLO 750
 #ifndef XT_POLY
 #define XT_POLY 0                                // of eight pairs of scores, how many go by the polynomial
 #endif
@@ -188,7 +202,8 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
     volatile int* abort = (volatile int*)(tmem_slot + 1);
     __shared__ float s_m[2 * XT_BM], s_l[2 * XT_BM];
     __shared__ int2 s_range[2 * XT_BM];
-    __shared__ int s_first, s_last;
+    __shared__ int s_to[2 * XT_BM];                                 // where a row's result begins, from the block's first token on; -1: no row
+    __shared__ int s_seen[2][8];                                    // [first, end) that each warp's rows see
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     PDL_ENTER_EARLY();
     CrossArgs a = arg.a;
@@ -198,22 +213,21 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
     const int r = arg.first_request + blockIdx.x / arg.max_pairs, pair = blockIdx.x % arg.max_pairs, kh = blockIdx.y;
     const int rank = blockIdx.z, cluster = gridDim.z, G = a.G, per_tile = XT_BM / G;
     const int tok0 = a.cu_tokens[r] + pair * 2 * per_tile, left = a.cu_tokens[r + 1] - tok0;
+    const int source = a.lens[r];
     if (left <= 0) return;                                          // (all blocks of a cluster)
     if ((smem_u32(smem) & 1023u) != 0) { if (tid == 0) atomicExch(error_flag, 40); return; }
     // Where the rows fit one tile, both halves of the block work on it: B has the same rows and the blocks of odd number, A those of even number.
     const bool two = left > per_tile;
-    const int len = max(0, min(a.lens[r], a.max_pages << a.page_shift));
+    const int len = max(0, min(source, a.max_pages << a.page_shift));
     const int* table = a.block_table + (size_t)r * a.max_pages;
     if (tid == 0) {
         mbar_init(q_full, 1); mbar_init(&drained[0], 1); mbar_init(&drained[1], 1);
         for (int i = 0; i < 4; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1); }
         for (int i = 0; i < XT_STAGES; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_free[i], two ? 2 : 1); mbar_init(&v_full[i], 1); mbar_init(&v_free[i], two ? 2 : 1); }
         *abort = 0;
-        s_first = len; s_last = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 0) { __syncwarp(); tmem_alloc<false>(tmem_slot, XT_TMEM); }
-    __syncthreads();
+    if (warp == 11) { __syncwarp(); tmem_alloc<false>(tmem_slot, XT_TMEM); }
     // this thread's row (threads 0..255): tile, token, head
     const int tile = warp >> 2, in_tile = tid & (XT_BM - 1), my_tok = (two ? tile * per_tile : 0) + in_tile / G, my_head = kh * G + in_tile % G;
     const bool mine = warp < 8 && in_tile < per_tile * G && my_tok < left;
@@ -221,14 +235,27 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
     if (mine) range = cross_range(a, tok0 + my_tok, len);
     if (warp < 8) {
         s_range[tid] = range;
-        if (a.spans == nullptr) { if (tid == 0) { s_first = 0; s_last = len; } }
-        else if (range.y > range.x) { atomicMin(&s_first, range.x); atomicMax(&s_last, range.y); }
+        s_to[tid] = mine ? (my_tok * a.K * G + my_head) * D : -1;
+        const int lowest = __reduce_min_sync(0xffffffffu, range.y > range.x ? range.x : len), highest = __reduce_max_sync(0xffffffffu, range.y);
+        if (lane == 0) { s_seen[0][warp] = lowest; s_seen[1][warp] = highest; }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = *tmem_slot;
-    const int first_block = s_first / XT_BN, blocks_all = s_last > s_first ? (s_last + XT_BN - 1) / XT_BN - first_block : 0;
+    int first_seen = s_seen[0][0], end_seen = s_seen[1][0];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) { first_seen = min(first_seen, s_seen[0][w]); end_seen = max(end_seen, s_seen[1][w]); }
+    const int first_block = first_seen / XT_BN, blocks_all = end_seen > first_seen ? (end_seen + XT_BN - 1) / XT_BN - first_block : 0;
+    bf16* const out0 = (bf16*)a.out + (size_t)tok0 * a.K * G * D;
+    if (blocks_all == 0) {                                          // nobody here sees anything: zeros (all blocks of a cluster come here)
+        if (warp == 11) { __syncwarp(); tmem_free<false>(tmem_base, XT_TMEM); }
+        for (int x = rank * XT_THREADS + tid; x < 2 * XT_BM * (D / 8); x += cluster * XT_THREADS) {
+            const int to = s_to[x / (D / 8)];
+            if (to >= 0 && (two || x < XT_BM * (D / 8))) reinterpret_cast<uint4*>(out0 + to)[x % (D / 8)] = make_uint4(0, 0, 0, 0);
+        }
+        return;
+    }
     const int share = (blocks_all + cluster - 1) / cluster;
     const int block0 = first_block + rank * share, nblk = max(0, min(share, blocks_all - rank * share));
 
@@ -242,11 +269,12 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
             uint64_t* freed = keys ? k_free : v_free;
             const int page = 1 << a.page_shift, rows = min(page, XT_BN), boxes = XT_BN / rows, box = lane % boxes, panel = lane / boxes;
             const bool loads = panel < NH;
-            auto row_of = [&](int i) -> int {                       // the box's first row among the cache's rows (past them: zeros)
-                const int key = (block0 + i) * XT_BN + box * rows;
-                if (!loads || i >= nblk || key >= len) return arg.cache_rows;
-                return (int)((((unsigned)table[key >> a.page_shift] * (unsigned)a.K + (unsigned)kh) << a.page_shift) + (unsigned)(key & (page - 1)));
+            // pages of 32 boxes, a lane a box, and of the 32 after them: looked up while the ones at hand are used
+            auto ids_at = [&](int x0) -> int {
+                const int x = x0 + lane, key = block0 * XT_BN + x * rows;
+                return x < nblk * boxes && key < len ? table[key >> a.page_shift] : -1;
             };
+            int ids_from = 0, ids = ids_at(0), ids_next = ids_at(32);
             if (keys && nblk > 0 && lane < NH * (two ? 2 : 1)) {
                 const int t = lane / NH, p = lane % NH;
                 if (lane == 0) mbar_expect_tx(q_full, (uint32_t)((two ? 2 : 1) * NH * per_tile * G * 128));
@@ -254,13 +282,16 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
                 tma_load_3d(sQ + t * XT_TILE + p * (XT_BM * 128), &map_q, p * 64, kh * G, tok0 + t * per_tile, q_full);
             }
             __syncwarp();
-            int from_row = row_of(0);
             bool ok = true;
             int asked = 0;
             for (int i = 0; ok && i < nblk; ++i) {
                 const int st = i % XT_STAGES;
                 if (i >= XT_STAGES) ok = warp_wait(&freed[st], ((i / XT_STAGES) - 1) & 1, abort, error_flag, 41);
                 if (!ok) break;
+                if (i * boxes - ids_from >= 32) { ids_from += 32; ids = ids_next; ids_next = ids_at(ids_from + 32); }
+                const int id = __shfl_sync(0xffffffffu, ids, i * boxes + box - ids_from);
+                // the box's first row among the cache's rows (past them: zeros)
+                const int from_row = id < 0 ? arg.cache_rows : (int)((((unsigned)id * (unsigned)a.K + (unsigned)kh) << a.page_shift) + (unsigned)(((block0 + i) * XT_BN + box * rows) & (page - 1)));
                 uint8_t* dst = (keys ? sK : sV) + st * XT_KV;
                 // the box that the source ends in: its values by plain stores, zeros from there on
                 const int tail = keys ? XT_BN : len - (block0 + i) * XT_BN, cut = tail < XT_BN ? tail / rows : boxes;
@@ -279,7 +310,6 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
                 if (lane == 0) mbar_expect_tx(&full[st], (uint32_t)(XT_KV - (partial ? NH * rows * 128 : 0)));
                 __syncwarp();
                 if (loads && !(partial && box == cut)) tma_load_2d(dst + panel * (XT_BN * 128) + box * rows * 128, map, panel * 64, from_row, &full[st]);
-                from_row = row_of(i + 1);
                 asked = i + 1;
             }
             // (what was asked for has to land before the block ends; where all went well the issuer has waited for it)
@@ -456,7 +486,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
             }
         }
         if (ok && (two || tile == 0)) {
-            bf16* dst = (bf16*)a.out + ((size_t)(tok0 + my_tok) * a.K * G + my_head) * D;
+            uint4* stage = reinterpret_cast<uint4*>(sQ + tile * XT_TILE);       // this tile's queries: its products are done
             const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
             const bool sees = range.y > range.x;
             bool odd = false;
@@ -476,7 +506,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
                 if (cluster > 1) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(sO + c * 16 + 4 * j) = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-                } else if (mine) {
+                } else {
                     uint32_t w[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
@@ -484,9 +514,21 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
                         odd |= !(fabsf(x) <= 3.0e38f) || !(fabsf(y) <= 3.0e38f);
                         asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[j]) : "f"(y), "f"(x));
                     }
-                    reinterpret_cast<uint4*>(dst)[c * 2] = make_uint4(w[0], w[1], w[2], w[3]);
-                    reinterpret_cast<uint4*>(dst)[c * 2 + 1] = make_uint4(w[4], w[5], w[6], w[7]);
+                    stage[XT_STAGED(in_tile, c * 2)] = make_uint4(w[0], w[1], w[2], w[3]);
+                    stage[XT_STAGED(in_tile, c * 2 + 1)] = make_uint4(w[4], w[5], w[6], w[7]);
                 }
+            }
+            if (cluster == 1) {
+                // a warp's rows out of shared memory, whole rows side by side (a thread its own row would touch 32 rows with every store)
+                __syncwarp();
+                constexpr int PIECES = D / 8, AT_ONCE = 32 / PIECES;
+                const int piece = lane % PIECES;
+#pragma unroll 4
+                for (int r0 = 0; r0 < 32; r0 += AT_ONCE) {
+                    const int rw = r0 + lane / PIECES, to = lane < AT_ONCE * PIECES && rw < 32 ? s_to[(tid & ~31) + rw] : -1;
+                    if (to >= 0) reinterpret_cast<uint4*>(out0 + to)[piece] = stage[XT_STAGED((tid & 96) + rw, piece)];
+                }
+                odd = odd && mine;
             }
             if (cluster > 1) { s_m[tid] = m_used; s_l[tid] = l_run; }
             if (a.spans != nullptr && cluster == 1) {
@@ -504,14 +546,14 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 0) { __syncwarp(); tmem_free<false>(tmem_base, XT_TMEM); }
+    if (warp == 11) { __syncwarp(); tmem_free<false>(tmem_base, XT_TMEM); }
     if (cluster > 1) {
         cross_cluster_sync();
         // block `rank` finishes rows rank, rank + cluster, ...: a warp a row, the partial results in rank order (all asked for before the first is used)
         const float* sO = (const float*)smem;
         for (int done = rank + warp * cluster; done < (two ? 2 * XT_BM : XT_BM); done += (XT_THREADS / 32) * cluster) {
-            const int in = done & (XT_BM - 1), tok = (done / XT_BM) * per_tile + in / G, head = kh * G + in % G;
-            if (in >= per_tile * G || tok >= left) continue;
+            const int to = s_to[done];
+            if (to < 0) continue;
             constexpr int PIECES = (D + 31) / 32;
             float w[XT_MAX_CLUSTER], u[XT_MAX_CLUSTER], part[XT_MAX_CLUSTER][PIECES], top = -INFINITY, sum = 0.0f, v[PIECES];
 #pragma unroll
@@ -536,7 +578,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
                 for (int x = 0; x < PIECES; ++x) v[x] = fmaf(f, part[c][x], v[x]);
             }
             const int2 rg = s_range[done];
-            bf16* dst = (bf16*)a.out + ((size_t)(tok0 + tok) * a.K * G + head) * D;
+            bf16* dst = out0 + to;
             bool odd = false;
 #pragma unroll
             for (int x = 0; x < PIECES; ++x) {
@@ -544,7 +586,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
                 odd |= !(fabsf(out) <= 3.0e38f);
                 if (x * 32 + lane < D) dst[x * 32 + lane] = __float2bfloat16_rn(out);
             }
-            if (a.spans != nullptr && __any_sync(0xffffffffu, odd)) { __syncwarp(); cross_row_alone<bf16>(arg.a, tok0 + tok, head, r, rg); }
+            if (a.spans != nullptr && __any_sync(0xffffffffu, odd)) { __syncwarp(); cross_row_alone<bf16>(arg.a, tok0 + to / (a.K * G * D), to / D % (a.K * G), r, rg); }
         }
         cross_cluster_sync();                                       // (a block's shared memory is read until here)
     }
@@ -574,12 +616,53 @@ static int map_queries(CUtensorMap* map, const void* q, long long stride, int H,
     return rc == CUDA_SUCCESS ? 0 : 1000 + (int)rc;
 }
 
+// How many clusters of so many blocks (one an SM) the device holds at once, asked once a device: clusters of eight leave SMs without one where an SM group has
+// no eight left (B200: 14 or so of the 18 that the SMs would make).
+static int clusters_at_once(int blocks) {
+    static int known[64][4];
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return 0;
+    const int which = blocks == 1 ? 0 : blocks == 2 ? 1 : blocks == 4 ? 2 : 3;
+    int n = device < 64 ? __atomic_load_n(&known[device][which], __ATOMIC_RELAXED) : 0;
+    if (n > 0) return n;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks * 148);
+    cfg.blockDim = dim3(XT_THREADS);
+    cfg.dynamicSmemBytes = XT_SMEM;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = blocks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, attention_cross_tc_kernel, &cfg) != cudaSuccess || n < 1) { cudaGetLastError(); n = 148 / blocks; }
+    if (blocks == 1 && n > 148) n = 148;
+    if (device < 64) __atomic_store_n(&known[device][which], n, __ATOMIC_RELAXED);
+    return n;
+}
+
+// Over how many blocks of a cluster a tile pair's keys are cut: the fewest rounds over the SMs, a round counted in cycles: a block's way in and out, a cluster's meeting,
+// and the blocks of 64 keys (both halves on the same rows: half as long each).
+static int choose_chunks(long long pairs, int longest, bool one_tile) {
+    const int keys = (longest + XT_BN - 1) / XT_BN;
+    int best = 1;
+    long long least = 0;
+    for (int c = 1; c <= XT_MAX_CLUSTER; c *= 2) {
+        if (c > 1 && keys < 4 * c) break;
+        const int room = clusters_at_once(c);
+        const long long rounds = (pairs + room - 1) / room, cost = rounds * (XT_COST_BLOCK + (c > 1 ? XT_COST_CLUSTER : 0) + (long long)((keys + c - 1) / c) * (one_tile ? XT_COST_SOLO : XT_COST_KEYS));
+        if (c == 1 || cost < least) { best = c; least = cost; }
+    }
+    return best;
+}
+
 // Pages of 16 to 128 positions; q, caches and out at 16 bytes, q_stride in whole 16-byte steps.
 MB_API int mb_attention_cross_tc(const CrossCall* c, cudaStream_t s) {
     if (c->requests <= 0 || c->max_query <= 0) return 0;
     const long long cache_rows = c->cache_pages * c->K * c->page_size;
     if (!cross_call_fits(c) || c->d != D || c->dtype != MB_BF16 || c->page_size < 16 || c->page_size > 128 || c->H / c->K > XT_BM || cache_rows <= 0 || cache_rows > 0x7fffff00LL ||
-        (((uintptr_t)c->q | (uintptr_t)c->k_cache | (uintptr_t)c->v_cache | (uintptr_t)c->out) & 15) != 0 || c->q_stride % 8 != 0 || !chunks_fit(c->chunks))
+        (((uintptr_t)c->q | (uintptr_t)c->k_cache | (uintptr_t)c->v_cache | (uintptr_t)c->out) & 15) != 0 || c->q_stride % 8 != 0 || (c->chunks != 0 && !chunks_fit(c->chunks)) ||
+        (long long)c->H * D * 2 * XT_BM > 0x7fffffffLL)
         return MB_ERR_BAD_SIZE;
     const int G = c->H / c->K, per_tile = XT_BM / G;
     const long long pairs = (c->max_query + 2LL * per_tile - 1) / (2 * per_tile);
@@ -587,11 +670,14 @@ MB_API int mb_attention_cross_tc(const CrossCall* c, cudaStream_t s) {
     static LaunchSmem allowed;
     int rc = allowed.allow(attention_cross_tc_kernel, XT_SMEM);
     if (rc != 0) return rc;
+    // (requests of unlike lengths: no more pairs than their tokens fill, and one more each)
+    const long long filled = c->requests + (long long)c->tokens / (2 * per_tile), most = pairs * c->requests < filled ? pairs * c->requests : filled;
+    const int chunks = c->chunks != 0 ? c->chunks : choose_chunks(most * c->K, c->longest, c->max_query <= per_tile);
     CUtensorMap mq, mk, mv;
     const int box_rows = c->page_size < XT_BN ? c->page_size : XT_BN;
     if ((rc = map_queries(&mq, c->q, c->q_stride, c->H, c->tokens, G, per_tile)) != 0) return rc;
     if ((rc = map_rows(&mk, c->k_cache, (uint64_t)cache_rows, (uint32_t)box_rows)) != 0) return rc;
     if ((rc = map_rows(&mv, c->v_cache, (uint64_t)cache_rows, (uint32_t)box_rows)) != 0) return rc;
     const CrossTc arg = {cross_args(c), c->error_flag, c->first, (int)pairs, (int)cache_rows};
-    return launch_kernel(attention_cross_tc_kernel, dim3((unsigned)(c->requests * pairs), c->K, c->chunks), dim3(XT_THREADS), XT_SMEM, s, c->chunks, mq, mk, mv, arg);
+    return launch_kernel(attention_cross_tc_kernel, dim3((unsigned)(c->requests * pairs), c->K, chunks), dim3(XT_THREADS), XT_SMEM, s, chunks, mq, mk, mv, arg);
 }

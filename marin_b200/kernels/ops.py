@@ -2995,16 +2995,8 @@ def _cross_lib(which: str, d: int):
     return lib
 
 
-def cross_chunks(blocks: int, longest: int) -> int:
-    """Over how many blocks of a cluster (1, 2, 4 or 8) a tile pair's keys are cut: as many as fill the SMs, none with fewer than 256 keys."""
-    chunks = 1
-    while chunks < 8 and blocks * chunks * 2 <= SM_COUNT and chunks * 256 < longest:
-        chunks *= 2
-    return chunks
-
-
 def cross_decode_chunks(pairs: int, longest: int) -> int:
-    """The same for single tokens (``pairs`` requests times kv heads): while there are fewer blocks than SMs, and once more for long sources that leave the SMs with few
+    """Over how many blocks of a cluster (1, 2, 4 or 8) a single token's keys are cut, ``pairs`` requests times kv heads: more while there are fewer blocks than SMs, and once more for long sources that leave the SMs with few
     blocks of unlike lengths.  (B200, heads of 128, 1 to 8 blocks each: 64 requests of 500 to 4,100 positions 103, 97, 105 and 143 us, of 577 all 31, 43, 60 and 92;
     8 of 4,096 44, 29, 28 and 30; 2 of 2,000 to 4,096 36, 21, 13 and 10.)"""
     chunks = 1
@@ -3042,7 +3034,7 @@ def attention_cross(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise KernelError(f"attention_cross: scale is a positive number, got {scale}")
     if T == 0 or R == 0:
         return
-    longest, group = max(0, int(source.longest)), H // K
+    longest = max(0, int(source.longest))
     at = (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr())
     aligned = stride % 8 == 0 and (at[0] | at[1] | at[2] | at[3]) % 16 == 0
     where = (table.data_ptr(), lens.data_ptr(), cu.data_ptr(), _address(spans), _scratch_for(q.device).error.data_ptr(), stride, pages, scale, _code(q), columns[1])
@@ -3056,8 +3048,7 @@ def attention_cross(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         if single and aligned and cross_decode_supported(dtype, H, K, d, page_size):
             fn, chunks, what = _packed_entry(f"mb_attention_cross_decode {d}", lambda: _cross_lib("decode", d)), cross_decode_chunks(n * K, longest), "attention_cross (single tokens)"
         elif aligned and cross_tc_supported(dtype, H, K, d, page_size) and 0 < pages * K * page_size < 0x7fffff00:
-            pairs = -(-most // (2 * (128 // group)))
-            fn, chunks, what = _packed_entry(f"mb_attention_cross_tc {d}", lambda: _cross_lib("tc", d)), cross_chunks(min(n * pairs, n + T * group // 256) * K, longest), "attention_cross (tensor cores)"
+            fn, chunks, what = _packed_entry(f"mb_attention_cross_tc {d}", lambda: _cross_lib("tc", d)), 0, "attention_cross (tensor cores)"
         else:
             fn, chunks, what = _packed_entry("mb_attention_cross", lambda: _lib("mb_attention_cross")), 0, "attention_cross"
         _check(fn(_CROSS.pack(*at, *where, first, n, most, T, chunks, longest, H, K, d, page_size), stream), what)
