@@ -199,32 +199,24 @@ __global__ void __launch_bounds__(256) attention_cross_kernel(const __grid_const
     const int warp = tid >> 5, lane = tid & 31;
     for (int row = rank + warp * (int)gridDim.z; row < BM; row += 8 * (int)gridDim.z) {
         if (row0 + row >= rows) break;
-        float w[CX_CHUNKS], top = -INFINITY, sum = 0.0f;
-#pragma unroll
-        for (int c = 0; c < CX_CHUNKS; ++c) {
-            w[c] = c < chunks ? (gridDim.z > 1 ? cross_peer((uint32_t)__cvta_generic_to_shared(&s_m[row]), c) : s_m[row]) : -INFINITY;
-            top = fmaxf(top, w[c]);
-        }
-        const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-        for (int c = 0; c < CX_CHUNKS; ++c) {
-            if (c >= chunks) continue;
-            w[c] = exp2f(w[c] - base);
-            sum += w[c] * (gridDim.z > 1 ? cross_peer((uint32_t)__cvta_generic_to_shared(&s_l[row]), c) : s_l[row]);
-        }
+        const bool sees = s_hi[row] > s_lo[row];
+        float sum = s_l[row], factor = 1.0f;
+        if (gridDim.z > 1) factor = cross_factor<true>(&s_m[row], &s_l[row], chunks, sum);
         const int t = t0 + (row0 + row) / a.G, head = kh * a.G + (row0 + row) % a.G;
         T* out = (T*)a.out + ((size_t)t * H + head) * a.d;
         bool odd = false;
-        for (int c = lane; c < a.d; c += 32) {
-            float v = 0.0f;
-#pragma unroll
-            for (int z = 0; z < CX_CHUNKS; ++z)
-                if (z < chunks) v = fmaf(w[z], gridDim.z > 1 ? cross_peer((uint32_t)__cvta_generic_to_shared(sQ + row * LD + c), z) : sQ[row * LD + c], v);
-            v = s_hi[row] > s_lo[row] ? v / sum : 0.0f;
-            odd |= !(fabsf(v) <= 3.0e38f);
-            out[c] = from_f32<T>(v);
+        for (int c0 = 0; c0 < a.d; c0 += 128) {
+            const int c = c0 + 4 * lane;
+            const float* from = sQ + row * LD + min(c, LD - 4);
+            float4 v = gridDim.z > 1 ? cross_join4(from, factor, chunks) : *reinterpret_cast<const float4*>(from);
+            v = sees ? make_float4(v.x / sum, v.y / sum, v.z / sum, v.w / sum) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            odd |= c < a.d && not_finite(v);
+            if (c < a.d) out[c] = from_f32<T>(v.x);
+            if (c + 1 < a.d) out[c + 1] = from_f32<T>(v.y);
+            if (c + 2 < a.d) out[c + 2] = from_f32<T>(v.z);
+            if (c + 3 < a.d) out[c + 3] = from_f32<T>(v.w);
         }
-        if (a.spans != nullptr && __any_sync(0xffffffffu, odd)) cross_row_alone<T>(arg, t, head, r, make_int2(s_lo[row], s_hi[row]));
+        if (a.spans != nullptr && __any_sync(0xffffffffu, odd)) { __syncwarp(); cross_row_alone<T>(arg, t, head, r, make_int2(s_lo[row], s_hi[row])); }
     }
     if (gridDim.z > 1) cross_cluster_sync();                        // (a block's shared memory is read until here)
 }

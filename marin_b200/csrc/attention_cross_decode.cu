@@ -194,27 +194,17 @@ __global__ void __launch_bounds__(XD_WARPS * 32) attention_cross_decode_kernel(C
     }
     if (cluster == 1) return;
     cross_cluster_sync();
-    for (int x = rank * XD_WARPS * 32 + threadIdx.x; x < G * D; x += cluster * XD_WARPS * 32) {
-        const int row = x / D;
-        float f[XD_MAX_CLUSTER], u[XD_MAX_CLUSTER], part[XD_MAX_CLUSTER], top = -INFINITY, sum = 0.0f, v = 0.0f;
-#pragma unroll
-        for (int c = 0; c < XD_MAX_CLUSTER; ++c) {
-            const int from = c < cluster ? c : 0;
-            f[c] = cross_peer((uint32_t)__cvta_generic_to_shared(&c_m[row]), from);
-            u[c] = cross_peer((uint32_t)__cvta_generic_to_shared(&c_l[row]), from);
-            part[c] = cross_peer((uint32_t)__cvta_generic_to_shared(&c_o[x]), from);
+    for (int row = rank + warp * cluster; row < G; row += XD_WARPS * cluster) {             // a warp a row, four columns a lane
+        float sum;
+        const float factor = cross_factor<false>(&c_m[row], &c_l[row], cluster, sum);
+        const float4 v = cross_join4(c_o + row * D + min(4 * lane, D - 4), factor, cluster);
+        const bool sees = range.y > range.x;
+        if (4 * lane < D) {
+            uint2 w;
+            w.x = pack_bf16(sees ? v.x / sum : 0.0f, sees ? v.y / sum : 0.0f);
+            w.y = pack_bf16(sees ? v.z / sum : 0.0f, sees ? v.w / sum : 0.0f);
+            reinterpret_cast<uint2*>((bf16*)a.out + ((size_t)t * a.K * G + kh * G + row) * D)[lane] = w;
         }
-#pragma unroll
-        for (int c = 0; c < XD_MAX_CLUSTER; ++c) if (c < cluster) top = fmaxf(top, f[c]);
-        const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-        for (int c = 0; c < XD_MAX_CLUSTER; ++c)
-            if (c < cluster) {
-                const float w = xd_exp2(f[c] - base);
-                sum = fmaf(w, u[c], sum);
-                v = fmaf(w, part[c], v);
-            }
-        ((bf16*)a.out)[((size_t)t * a.K * G + kh * G) * D + x] = __float2bfloat16_rn(range.y > range.x ? v / sum : 0.0f);
     }
     cross_cluster_sync();                                           // (a block's shared memory is read until here)
 }
@@ -222,8 +212,8 @@ __global__ void __launch_bounds__(XD_WARPS * 32) attention_cross_decode_kernel(C
 // Requests of one token each.
 MB_API int mb_attention_cross_decode(const CrossCall* c, cudaStream_t s) {
     if (c->requests <= 0) return 0;
-    if (!cross_call_fits(c) || c->d != D || c->dtype != MB_BF16 || c->page_size < XD_KEYS || c->H / c->K > 8 || (((uintptr_t)c->q | (uintptr_t)c->out) & 3) != 0 || c->q_stride % 2 != 0 ||
-        (((uintptr_t)c->k_cache | (uintptr_t)c->v_cache) & 15) != 0 || !chunks_fit(c->chunks))
+    if (!cross_call_fits(c) || c->d != D || c->dtype != MB_BF16 || c->page_size < XD_KEYS || c->H / c->K > 8 || ((uintptr_t)c->q & 3) != 0 || ((uintptr_t)c->out & 7) != 0 || c->q_stride % 2 != 0 ||
+        (((uintptr_t)c->k_cache | (uintptr_t)c->v_cache) & 15) != 0 || !chunks_fit(c->chunks) || c->chunks > XD_MAX_CLUSTER)
         return MB_ERR_BAD_SIZE;
     static LaunchSmem allowed;
     const int rc = allowed.allow(attention_cross_decode_kernel, XD_SMEM);

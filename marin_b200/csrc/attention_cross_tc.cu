@@ -33,7 +33,6 @@ static_assert(HEAD_DIM % 16 == 0 && HEAD_DIM >= 16 && HEAD_DIM <= 128, "heads in
 #define XT_BN 64                                 // keys of a block
 #define XT_TILE (NH * XT_BM * 128)               // bytes of a tile of queries
 #define XT_KV (NH * XT_BN * 128)                 // bytes of a block of keys, or of values
-#define XT_STAGES 4                             // blocks of keys, and of values, on their way
 #define XT_OLD (D + 4)                           // floats between rows of O for the cluster
 #define XT_BARS 512
 // 16-byte piece c of row r of a tile's results in shared memory: rows of whole 128 bytes swizzled, others a piece apart, so that neither a thread's row nor a
@@ -43,20 +42,19 @@ static_assert(HEAD_DIM % 16 == 0 && HEAD_DIM >= 16 && HEAD_DIM <= 128, "heads in
 #else
 #define XT_STAGED(r, c) ((r) * (D / 8 + 1) + (c))
 #endif
-#define XT_SMEM (2 * XT_TILE + 2 * XT_STAGES * XT_KV + XT_BARS)
-static_assert(2 * XT_BM * XT_OLD * 4 <= 2 * XT_TILE + 2 * XT_STAGES * XT_KV, "partial results fit the tiles' memory");
 static_assert(D % 64 == 0 || XT_BM * (D * 2 + 16) <= XT_TILE, "a tile's results fit its queries' memory");
-static_assert(XT_BM * (D % 64 == 0 ? D * 2 : D * 2 + 16) <= XT_BM * XT_OLD * 4, "and lie ahead of B's partial results");
-static_assert(XT_SMEM <= 232448 - 6144, "static shared memory is beside it");
-#define XT_TMEM 512                              // two S buffers of A, of B (64 columns each), O of A, O of B (128)
-#define XT_O_COL 256
-#define XT_THREADS 384
-#define XT_MAX_CLUSTER 8
-// cycles: a block's way in and out, a cluster's meeting, 64 keys of two tiles, of one (see choose_chunks)
+#define XT_STAGES (NH == 1 ? 4 : 2)              // blocks of keys, and of values, on their way
+#define XT_SMEM (XT_TILE + 2 * XT_STAGES * XT_KV + XT_BARS)
+#define XT_TMEM 256                              // two buffers of scores (64 columns each), then O
+#define XT_O_COL 128
+#define XT_THREADS 256                           // warps 0..3 the rows, 4 loads Q and K, 5 V, 6 issues the products
+static_assert(XT_BM * XT_OLD * 4 <= XT_TILE + 2 * XT_STAGES * XT_KV, "partial results fit the tile's memory");
+static_assert(2 * (XT_SMEM + 1024 + XT_BM * 20 + 512) <= 233472, "two blocks an SM");
+#define XT_MAX_CLUSTER 16                        // (more than 8 is a size the device may refuse)
+// cycles: a block's way in and out, a cluster's meeting, 64 keys (see choose_chunks)
 #define XT_COST_BLOCK 9000
 #define XT_COST_CLUSTER 4000
 #define XT_COST_KEYS 1400
-#define XT_COST_SOLO 750
 #ifndef XT_POLY
 #define XT_POLY 0                                // of eight pairs of scores, how many go by the polynomial
 #endif
@@ -64,7 +62,7 @@ static_assert(XT_SMEM <= 232448 - 6144, "static shared memory is beside it");
 struct CrossTc {
     CrossArgs a;
     int* error_flag;
-    int first_request, max_pairs, cache_rows;
+    int first_request, max_tiles, cache_rows;
 };
 
 __device__ __forceinline__ float xt_exp2(float x) {
@@ -182,58 +180,61 @@ __device__ __forceinline__ void umma_bf16_tmem_a(uint32_t tmem_d, uint32_t tmem_
         : "memory");
 }
 
-__global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+__global__ void __launch_bounds__(XT_THREADS, 2) attention_cross_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CrossTc arg) {
     extern __shared__ __align__(1024) uint8_t smem[];
-    uint8_t* sQ = smem;                                             // [tile][panel][128 rows][128 B]
-    uint8_t* sK = sQ + 2 * XT_TILE;                                 // [stage][panel][128 rows][128 B]
+    uint8_t* sQ = smem;                                             // [panel][128 rows][128 B]
+    uint8_t* sK = sQ + XT_TILE;                                 // [stage][panel][128 rows][128 B]
     uint8_t* sV = sK + XT_STAGES * XT_KV;
     uint64_t* bars = (uint64_t*)(sV + XT_STAGES * XT_KV);
     uint64_t* q_full = bars;
-    uint64_t* s_full = bars + 1;                                    // [tile][buffer] scores are there
-    uint64_t* p_full = bars + 5;                                    // [tile][buffer] weights are there (four warps arrive)
-    uint64_t* o_done = bars + 9;                                    // [tile][buffer] P V of the buffer's weights is done
-    uint64_t* drained = bars + 13;
-    uint64_t* k_full = bars + 15;                                   // [stage]
+    uint64_t* s_full = bars + 1;                                    // [buffer] scores are there
+    uint64_t* p_full = bars + 3;                                    // [buffer] weights are there (four warps arrive)
+    uint64_t* o_done = bars + 5;                                    // [buffer] P V of the buffer's weights is done
+    uint64_t* drained = bars + 7;
+    uint64_t* k_full = bars + 8;                                    // [stage]
     uint64_t* k_free = k_full + XT_STAGES;
     uint64_t* v_full = k_free + XT_STAGES;
     uint64_t* v_free = v_full + XT_STAGES;
     uint32_t* tmem_slot = (uint32_t*)(v_free + XT_STAGES);
     volatile int* abort = (volatile int*)(tmem_slot + 1);
-    __shared__ float s_m[2 * XT_BM], s_l[2 * XT_BM];
-    __shared__ int2 s_range[2 * XT_BM];
-    __shared__ int s_to[2 * XT_BM];                                 // where a row's result begins, from the block's first token on; -1: no row
-    __shared__ int s_seen[2][8];                                    // [first, end) that each warp's rows see
+    __shared__ float s_m[XT_BM], s_l[XT_BM];
+    __shared__ int2 s_range[XT_BM];
+    __shared__ int s_to[XT_BM];                                 // where a row's result begins, from the block's first token on; -1: no row
+    __shared__ int s_seen[2][4];                                    // [first, end) that each warp's rows see
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     PDL_ENTER_EARLY();
     CrossArgs a = arg.a;
     a.q = pdl_fresh((const char*)a.q); a.v_cache = pdl_fresh((const char*)a.v_cache); a.k_cache = pdl_fresh((const char*)a.k_cache);
     a.block_table = pdl_fresh(a.block_table); a.lens = pdl_fresh(a.lens); a.cu_tokens = pdl_fresh(a.cu_tokens); a.spans = pdl_fresh(a.spans);
     int* error_flag = arg.error_flag;
-    const int r = arg.first_request + blockIdx.x / arg.max_pairs, pair = blockIdx.x % arg.max_pairs, kh = blockIdx.y;
+    const int r = arg.first_request + blockIdx.x / arg.max_tiles, number = blockIdx.x % arg.max_tiles, kh = blockIdx.y;
     const int rank = blockIdx.z, cluster = gridDim.z, G = a.G, per_tile = XT_BM / G;
-    const int tok0 = a.cu_tokens[r] + pair * 2 * per_tile, left = a.cu_tokens[r + 1] - tok0;
+    const int tok0 = a.cu_tokens[r] + number * per_tile, left = a.cu_tokens[r + 1] - tok0;
     const int source = a.lens[r];
     if (left <= 0) return;                                          // (all blocks of a cluster)
     if ((smem_u32(smem) & 1023u) != 0) { if (tid == 0) atomicExch(error_flag, 40); return; }
-    // Where the rows fit one tile, both halves of the block work on it: B has the same rows and the blocks of odd number, A those of even number.
-    const bool two = left > per_tile;
     const int len = max(0, min(source, a.max_pages << a.page_shift));
     const int* table = a.block_table + (size_t)r * a.max_pages;
-    if (tid == 0) {
-        mbar_init(q_full, 1); mbar_init(&drained[0], 1); mbar_init(&drained[1], 1);
-        for (int i = 0; i < 4; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1); }
-        for (int i = 0; i < XT_STAGES; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_free[i], two ? 2 : 1); mbar_init(&v_full[i], 1); mbar_init(&v_free[i], two ? 2 : 1); }
-        *abort = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (warp == 4) {                                                // (the queries are asked for at once; the keys' range is not known yet)
+        if (lane == 0) {
+            mbar_init(q_full, 1); mbar_init(drained, 1);
+            for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1); }
+            for (int i = 0; i < XT_STAGES; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_free[i], 1); mbar_init(&v_full[i], 1); mbar_init(&v_free[i], 1); }
+            *abort = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            mbar_expect_tx(q_full, (uint32_t)(NH * per_tile * G * 128));
+            for (int p = 0; p < NH; ++p) tma_load_3d(sQ + p * (XT_BM * 128), &map_q, p * 64, kh * G, tok0, q_full);
+        }
+        __syncwarp();
     }
-    if (warp == 11) { __syncwarp(); tmem_alloc<false>(tmem_slot, XT_TMEM); }
-    // this thread's row (threads 0..255): tile, token, head
-    const int tile = warp >> 2, in_tile = tid & (XT_BM - 1), my_tok = (two ? tile * per_tile : 0) + in_tile / G, my_head = kh * G + in_tile % G;
-    const bool mine = warp < 8 && in_tile < per_tile * G && my_tok < left;
+    if (warp == 7) { __syncwarp(); tmem_alloc<false>(tmem_slot, XT_TMEM); }
+    // this thread's row (the first threads): tile, token, head
+    const int my_tok = tid / G, my_head = kh * G + tid % G;
+    const bool mine = tid < per_tile * G && my_tok < left;
     int2 range = make_int2(0, 0);
     if (mine) range = cross_range(a, tok0 + my_tok, len);
-    if (warp < 8) {
+    if (warp < 4) {
         s_range[tid] = range;
         s_to[tid] = mine ? (my_tok * a.K * G + my_head) * D : -1;
         const int lowest = __reduce_min_sync(0xffffffffu, range.y > range.x ? range.x : len), highest = __reduce_max_sync(0xffffffffu, range.y);
@@ -245,14 +246,15 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
     const uint32_t tmem_base = *tmem_slot;
     int first_seen = s_seen[0][0], end_seen = s_seen[1][0];
 #pragma unroll
-    for (int w = 1; w < 8; ++w) { first_seen = min(first_seen, s_seen[0][w]); end_seen = max(end_seen, s_seen[1][w]); }
+    for (int w = 1; w < 4; ++w) { first_seen = min(first_seen, s_seen[0][w]); end_seen = max(end_seen, s_seen[1][w]); }
     const int first_block = first_seen / XT_BN, blocks_all = end_seen > first_seen ? (end_seen + XT_BN - 1) / XT_BN - first_block : 0;
     bf16* const out0 = (bf16*)a.out + (size_t)tok0 * a.K * G * D;
     if (blocks_all == 0) {                                          // nobody here sees anything: zeros (all blocks of a cluster come here)
-        if (warp == 11) { __syncwarp(); tmem_free<false>(tmem_base, XT_TMEM); }
-        for (int x = rank * XT_THREADS + tid; x < 2 * XT_BM * (D / 8); x += cluster * XT_THREADS) {
+        if (warp == 7) { __syncwarp(); tmem_free<false>(tmem_base, XT_TMEM); }
+        mbar_wait(q_full, 0);                                       // (what was asked for has to land)
+        for (int x = rank * XT_THREADS + tid; x < XT_BM * (D / 8); x += cluster * XT_THREADS) {
             const int to = s_to[x / (D / 8)];
-            if (to >= 0 && (two || x < XT_BM * (D / 8))) reinterpret_cast<uint4*>(out0 + to)[x % (D / 8)] = make_uint4(0, 0, 0, 0);
+            if (to >= 0) reinterpret_cast<uint4*>(out0 + to)[x % (D / 8)] = make_uint4(0, 0, 0, 0);
         }
         return;
     }
@@ -260,10 +262,10 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
     const int block0 = first_block + rank * share, nblk = max(0, min(share, blocks_all - rank * share));
 
     const int role = warp_same(warp);                               // (the branches are then the same in all lanes for the compiler too: see elect_one)
-    if (role >= 8) {
-        if (role == 8 || role == 9) {
+    if (role >= 4) {
+        if (role == 4 || role == 5) {
             // ---- the loaders: a lane a box (a page's rows of one panel), as soon as the block's buffer is free; where the boxes lie is looked up a block ahead ----
-            const bool keys = role == 8;
+            const bool keys = role == 4;
             const CUtensorMap* map = keys ? &map_k : &map_v;
             uint64_t* full = keys ? k_full : v_full;
             uint64_t* freed = keys ? k_free : v_free;
@@ -275,12 +277,6 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
                 return x < nblk * boxes && key < len ? table[key >> a.page_shift] : -1;
             };
             int ids_from = 0, ids = ids_at(0), ids_next = ids_at(32);
-            if (keys && nblk > 0 && lane < NH * (two ? 2 : 1)) {
-                const int t = lane / NH, p = lane % NH;
-                if (lane == 0) mbar_expect_tx(q_full, (uint32_t)((two ? 2 : 1) * NH * per_tile * G * 128));
-                __syncwarp(__activemask());
-                tma_load_3d(sQ + t * XT_TILE + p * (XT_BM * 128), &map_q, p * 64, kh * G, tok0 + t * per_tile, q_full);
-            }
             __syncwarp();
             bool ok = true;
             int asked = 0;
@@ -315,39 +311,36 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
             // (what was asked for has to land before the block ends; where all went well the issuer has waited for it)
             if (!ok)
                 for (int i = max(0, asked - XT_STAGES); i < asked; ++i) mbar_wait_warp(&full[i % XT_STAGES], (i / XT_STAGES) & 1);
-        } else {
-            // ---- the issuers, one a tile: what one spends on its barriers is time in which the other's products run ----
+        } else if (role == 6) {
+            // ---- the issuer ----
             constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(XT_BN >> 3) << 17) | ((uint32_t)(XT_BM >> 4) << 24);
             constexpr uint32_t idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(XT_BM >> 4) << 24);
-            const uint32_t elected = elect_one(), t = (uint32_t)(role - 10), tmem = warp_same(tmem_base);
-            const uint32_t tmem_s = tmem + t * 128, tmem_o = tmem + XT_O_COL + t * 128;
-            const int both = warp_same((int)two), blocks = both ? warp_same(nblk) : (warp_same(nblk) + 1 - (int)t) >> 1;
-            auto block = [&](int i) { return both ? i : 2 * i + (int)t; };    // number i of this issuer's blocks
-            uint64_t *s_bar = s_full + 2 * t, *p_bar = p_full + 2 * t, *o_bar = o_done + 2 * t;
-            const uint64_t qdesc = umma_desc(smem_u32(sQ) + (both ? t * XT_TILE : 0u));
+            const uint32_t elected = elect_one(), tmem_s = warp_same(tmem_base), tmem_o = tmem_s + XT_O_COL;
+            const int blocks = warp_same(nblk);
+            const uint64_t qdesc = umma_desc(smem_u32(sQ));
             auto scores = [&](int i) {
-                const int st = block(i) % XT_STAGES;
+                const int st = i % XT_STAGES;
                 const uint64_t kdesc = umma_desc(smem_u32(sK) + st * XT_KV);
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk)
                     umma_bf16(tmem_s + (uint32_t)((i & 1) * XT_BN), qdesc + (uint32_t)((kk / 4) * (XT_BM * 128 >> 4) + 2 * (kk % 4)),
                               kdesc + (uint32_t)((kk / 4) * (XT_BN * 128 >> 4) + 2 * (kk % 4)), idesc_s, kk > 0 ? 1u : 0u, elected);
-                umma_commit(&s_bar[i & 1], elected);
+                umma_commit(&s_full[i & 1], elected);
                 umma_commit(&k_free[st], elected);
             };
             bool ok = blocks > 0 && warp_wait(q_full, 0, abort, error_flag, 42);
             for (int i = 0; ok && i < min(2, blocks); ++i) {
-                ok = warp_wait(&k_full[block(i) % XT_STAGES], (block(i) / XT_STAGES) & 1, abort, error_flag, 42);
+                ok = warp_wait(&k_full[i % XT_STAGES], (i / XT_STAGES) & 1, abort, error_flag, 42);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 scores(i);
             }
             for (int i = 0; ok && i < blocks; ++i) {
-                const int st = block(i) % XT_STAGES, next = block(i + 2);
+                const int st = i % XT_STAGES, next = i + 2;
                 const bool more = i + 2 < blocks;
-                ok = warp_wait(&v_full[st], (block(i) / XT_STAGES) & 1, abort, error_flag, 43);
+                ok = warp_wait(&v_full[st], (i / XT_STAGES) & 1, abort, error_flag, 43);
                 if (ok && more) ok = warp_wait(&k_full[next % XT_STAGES], (next / XT_STAGES) & 1, abort, error_flag, 45);
-                if (ok) ok = warp_wait(&p_bar[i & 1], (i >> 1) & 1, abort, error_flag, 44);
+                if (ok) ok = warp_wait(&p_full[i & 1], (i >> 1) & 1, abort, error_flag, 44);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint64_t vdesc = umma_desc_mn(smem_u32(sV) + st * XT_KV, XT_BN * 128);
@@ -355,27 +348,26 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
                 for (int kk = 0; kk < XT_BN / 16; ++kk)
                     umma_bf16_tmem_a(tmem_o, tmem_s + (uint32_t)((i & 1) * XT_BN + kk * 8), vdesc + (uint32_t)(kk * (2048 >> 4)), idesc_pv, (i > 0 || kk > 0) ? 1u : 0u, elected);
                 if (more) scores(i + 2);                            // (S goes where P lies: the tensor core takes an issuer's products in their order)
-                umma_commit(&o_bar[i & 1], elected);
+                umma_commit(&o_done[i & 1], elected);
                 umma_commit(&v_free[st], elected);
             }
             if (!ok && blocks > 0) {                                // (and what was issued has to end)
-                umma_commit(&drained[t], elected);
-                mbar_wait_warp(&drained[t], 0);
+                umma_commit(drained, elected);
+                mbar_wait_warp(drained, 0);
             }
         }
     } else {
         // ---- the rows ----
         const uint32_t lane_base = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
-        const uint32_t o_col = lane_base + (uint32_t)(XT_O_COL + tile * 128);
+        const uint32_t o_col = lane_base + XT_O_COL;
         const float sl2 = a.scale * 1.4426950408889634f;
         // (rows that are not there or see nothing: their results are not looked at, so their scores need no mask)
         const int mask_from = range.y > range.x ? range.x : -0x40000000, mask_to = range.y > range.x ? range.y : 0x7fffffff;
         float m_used = -INFINITY, l_run = 0.0f;
         bool ok = true;
-        const int steps = two ? nblk : (nblk + 1 - tile) >> 1;
-        for (int i = 0; i < steps; ++i) {
-            const uint32_t s_col = lane_base + (uint32_t)(tile * 128 + (i & 1) * XT_BN);
-            ok = warp_wait(&s_full[tile * 2 + (i & 1)], (i >> 1) & 1, abort, error_flag, 46);
+        for (int i = 0; i < nblk; ++i) {
+            const uint32_t s_col = lane_base + (uint32_t)((i & 1) * XT_BN);
+            ok = warp_wait(&s_full[i & 1], (i >> 1) & 1, abort, error_flag, 46);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             float s[XT_BN];
@@ -383,7 +375,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
             tmem_ld32_async(s_col + 32, s + 32);
             tmem_ld_wait(s);
             tmem_ld_wait(s + 32);
-            const int key0 = (block0 + (two ? i : 2 * i + tile)) * XT_BN, from = mask_from - key0, to = mask_to - key0;
+            const int key0 = (block0 + i) * XT_BN, from = mask_from - key0, to = mask_to - key0;
             if (__any_sync(0xffffffffu, from > 0 || to < XT_BN)) {
 #pragma unroll
                 for (int j = 0; j < XT_BN; ++j)
@@ -400,7 +392,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
             if (__any_sync(0xffffffffu, raise)) {
                 if (raise) { corr = xt_exp2(m_used - m_true); m_used = m_true; }
                 if (i > 0) {                                        // (P V of the blocks ahead has to be done; of the one before last it is, these scores came after it)
-                    ok = warp_wait(&o_done[tile * 2 + ((i - 1) & 1)], ((i - 1) >> 1) & 1, abort, error_flag, 47);
+                    ok = warp_wait(&o_done[(i - 1) & 1], ((i - 1) >> 1) & 1, abort, error_flag, 47);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
@@ -438,84 +430,52 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[tile * 2 + (i & 1)]);
+            if (lane == 0) mbar_arrive(&p_full[i & 1]);
             float u0, u1;
             of_pair(add_pair(sum2[0], sum2[1]), u0, u1);
             l_run = l_run * corr + (u0 + u1);
         }
         // (the polynomial makes a large number of a NaN: no sum of weights of at most 2^8 comes near it)
         if (!(l_run < 1.0e30f)) l_run = __int_as_float(0x7fc00000);
-        if (ok && steps > 0) ok = warp_wait(&o_done[tile * 2 + ((steps - 1) & 1)], ((steps - 1) >> 1) & 1, abort, error_flag, 47);
+        if (nblk == 0) warp_wait(q_full, 0, abort, error_flag, 42);     // (nothing to do in this block of a cluster: what was asked for has to land all the same)
+        if (ok && nblk > 0) ok = warp_wait(&o_done[(nblk - 1) & 1], ((nblk - 1) >> 1) & 1, abort, error_flag, 47);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const int others = two ? nblk : (nblk + tile) >> 1;         // blocks of the other half
         float* sO = (float*)smem + (size_t)tid * XT_OLD;
-        if (cluster > 1 || !two) {
-            // the tiles' memory is about to be written over: once every product of both halves is done
-            if (ok && others > 0) ok = warp_wait(&o_done[(1 - tile) * 2 + ((others - 1) & 1)], ((others - 1) >> 1) & 1, abort, error_flag, 47);
-            asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (cluster > 1) {
+            // the tile's memory is about to be written over: by now all products are done (this warp has seen it), and every warp of the rows says so
+            asm volatile("bar.sync 1, 128;" ::: "memory");
         }
-        // 16 columns of this row, or zeros where it had no block
-        auto load_o = [&](int c, float* o) {
-            if (steps > 0) {
-                tmem_ld16(o_col + c * 16, o);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) o[j] = 0.0f;
-            }
-        };
-        float mine_f = 1.0f, other_f = 0.0f;                        // what this half's and B's partial results are multiplied by
-        if (!two) {
-            if (tile == 1) {
-                s_m[tid] = m_used; s_l[tid] = l_run;
-                if (ok) {
-#pragma unroll
-                    for (int c = 0; c < D / 16; ++c) {
-                        float o[16];
-                        load_o(c, o);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(sO + c * 16 + 4 * j) = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-                    }
-                }
-            }
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            if (tile == 0) {
-                const float m_b = s_m[tid + XT_BM], top = fmaxf(m_used, m_b), base = top == -INFINITY ? 0.0f : top;
-                mine_f = xt_exp2(m_used - base); other_f = xt_exp2(m_b - base);
-                l_run = fmaf(mine_f, l_run, other_f * s_l[tid + XT_BM]);
-                m_used = top;
-            }
-        }
-        if (ok && (two || tile == 0)) {
-            uint4* stage = reinterpret_cast<uint4*>(sQ + tile * XT_TILE);       // this tile's queries: its products are done
+        if (ok) {
+            uint4* stage = reinterpret_cast<uint4*>(sQ);            // (the queries': the products are done)
             const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
             const bool sees = range.y > range.x;
             bool odd = false;
 #pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
-                float o[16];
-                load_o(c, o);
-                if (!two) {
-                    const float4* b = reinterpret_cast<const float4*>(sO + XT_BM * XT_OLD + c * 16);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float4 f = b[j];
-                        o[4 * j] = fmaf(mine_f, o[4 * j], other_f * f.x); o[4 * j + 1] = fmaf(mine_f, o[4 * j + 1], other_f * f.y);
-                        o[4 * j + 2] = fmaf(mine_f, o[4 * j + 2], other_f * f.z); o[4 * j + 3] = fmaf(mine_f, o[4 * j + 3], other_f * f.w);
-                    }
-                }
-                if (cluster > 1) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(sO + c * 16 + 4 * j) = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+            for (int c = 0; c < (D + 31) / 32; ++c) {               // 32 columns at a time (of the last ones what there is: tensor memory behind them is this block's own)
+                float o[32];
+                if (nblk > 0) {
+                    tmem_ld32_async(o_col + c * 32, o);
+                    tmem_ld_wait(o);
                 } else {
-                    uint32_t w[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float x = sees ? o[2 * j] * inv : 0.0f, y = sees ? o[2 * j + 1] * inv : 0.0f;
-                        odd |= !(fabsf(x) <= 3.0e38f) || !(fabsf(y) <= 3.0e38f);
-                        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[j]) : "f"(y), "f"(x));
+                    for (int j = 0; j < 32; ++j) o[j] = 0.0f;
+                }
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    if (c * 32 + h * 8 >= D) continue;
+                    if (cluster > 1) {
+                        *reinterpret_cast<float4*>(sO + c * 32 + h * 8) = make_float4(o[8 * h], o[8 * h + 1], o[8 * h + 2], o[8 * h + 3]);
+                        *reinterpret_cast<float4*>(sO + c * 32 + h * 8 + 4) = make_float4(o[8 * h + 4], o[8 * h + 5], o[8 * h + 6], o[8 * h + 7]);
+                    } else {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float x = sees ? o[8 * h + 2 * j] * inv : 0.0f, y = sees ? o[8 * h + 2 * j + 1] * inv : 0.0f;
+                            odd |= !(fabsf(x) <= 3.0e38f) || !(fabsf(y) <= 3.0e38f);
+                            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[j]) : "f"(y), "f"(x));
+                        }
+                        stage[XT_STAGED(tid, c * 4 + h)] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
-                    stage[XT_STAGED(in_tile, c * 2)] = make_uint4(w[0], w[1], w[2], w[3]);
-                    stage[XT_STAGED(in_tile, c * 2 + 1)] = make_uint4(w[4], w[5], w[6], w[7]);
                 }
             }
             if (cluster == 1) {
@@ -525,8 +485,8 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
                 const int piece = lane % PIECES;
 #pragma unroll 4
                 for (int r0 = 0; r0 < 32; r0 += AT_ONCE) {
-                    const int rw = r0 + lane / PIECES, to = lane < AT_ONCE * PIECES && rw < 32 ? s_to[(tid & ~31) + rw] : -1;
-                    if (to >= 0) reinterpret_cast<uint4*>(out0 + to)[piece] = stage[XT_STAGED((tid & 96) + rw, piece)];
+                    const int rw = r0 + lane / PIECES, to = lane < AT_ONCE * PIECES && rw < 32 ? s_to[warp * 32 + rw] : -1;
+                    if (to >= 0) reinterpret_cast<uint4*>(out0 + to)[piece] = stage[XT_STAGED(warp * 32 + rw, piece)];
                 }
                 odd = odd && mine;
             }
@@ -546,47 +506,27 @@ __global__ void __launch_bounds__(XT_THREADS, 1) attention_cross_tc_kernel(const
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 11) { __syncwarp(); tmem_free<false>(tmem_base, XT_TMEM); }
+    if (warp == 7) { __syncwarp(); tmem_free<false>(tmem_base, XT_TMEM); }
     if (cluster > 1) {
         cross_cluster_sync();
-        // block `rank` finishes rows rank, rank + cluster, ...: a warp a row, the partial results in rank order (all asked for before the first is used)
+        // block `rank` finishes rows rank, rank + cluster, ...: a warp a row, four columns a lane
         const float* sO = (const float*)smem;
-        for (int done = rank + warp * cluster; done < (two ? 2 * XT_BM : XT_BM); done += (XT_THREADS / 32) * cluster) {
+        for (int done = rank + warp * cluster; done < XT_BM; done += (XT_THREADS / 32) * cluster) {
             const int to = s_to[done];
             if (to < 0) continue;
-            constexpr int PIECES = (D + 31) / 32;
-            float w[XT_MAX_CLUSTER], u[XT_MAX_CLUSTER], part[XT_MAX_CLUSTER][PIECES], top = -INFINITY, sum = 0.0f, v[PIECES];
-#pragma unroll
-            for (int c = 0; c < XT_MAX_CLUSTER; ++c) {
-                const int from = c < cluster ? c : rank;
-                w[c] = cross_peer(smem_u32(&s_m[done]), from);
-                u[c] = cross_peer(smem_u32(&s_l[done]), from);
-#pragma unroll
-                for (int x = 0; x < PIECES; ++x) part[c][x] = cross_peer(smem_u32(sO + (size_t)done * XT_OLD + min(x * 32 + lane, D - 1)), from);
-            }
-#pragma unroll
-            for (int c = 0; c < XT_MAX_CLUSTER; ++c) top = fmaxf(top, w[c]);
-            const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-            for (int x = 0; x < PIECES; ++x) v[x] = 0.0f;
-#pragma unroll
-            for (int c = 0; c < XT_MAX_CLUSTER; ++c) {
-                if (c >= cluster) continue;
-                const float f = xt_exp2(w[c] - base);
-                sum = fmaf(f, u[c], sum);
-#pragma unroll
-                for (int x = 0; x < PIECES; ++x) v[x] = fmaf(f, part[c][x], v[x]);
-            }
+            float sum;
+            const float factor = cross_factor<false>(&s_m[done], &s_l[done], cluster, sum);
+            float4 v = cross_join4(sO + (size_t)done * XT_OLD + min(4 * lane, D - 4), factor, cluster);
             const int2 rg = s_range[done];
-            bf16* dst = out0 + to;
-            bool odd = false;
-#pragma unroll
-            for (int x = 0; x < PIECES; ++x) {
-                const float out = rg.y > rg.x && sum != 0.0f ? v[x] / sum : 0.0f;
-                odd |= !(fabsf(out) <= 3.0e38f);
-                if (x * 32 + lane < D) dst[x * 32 + lane] = __float2bfloat16_rn(out);
+            const float inv = rg.y > rg.x && sum != 0.0f ? 1.0f / sum : 0.0f;
+            v = inv == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+            if (4 * lane < D) {
+                uint2 w;
+                asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w.x) : "f"(v.y), "f"(v.x));
+                asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w.y) : "f"(v.w), "f"(v.z));
+                reinterpret_cast<uint2*>(out0 + to)[lane] = w;
             }
-            if (a.spans != nullptr && __any_sync(0xffffffffu, odd)) { __syncwarp(); cross_row_alone<bf16>(arg.a, tok0 + to / (a.K * G * D), to / D % (a.K * G), r, rg); }
+            if (a.spans != nullptr && __any_sync(0xffffffffu, not_finite(v))) { __syncwarp(); cross_row_alone<bf16>(arg.a, tok0 + to / (a.K * G * D), to / D % (a.K * G), r, rg); }
         }
         cross_cluster_sync();                                       // (a block's shared memory is read until here)
     }
@@ -619,14 +559,15 @@ static int map_queries(CUtensorMap* map, const void* q, long long stride, int H,
 // How many clusters of so many blocks (one an SM) the device holds at once, asked once a device: clusters of eight leave SMs without one where an SM group has
 // no eight left (B200: 14 or so of the 18 that the SMs would make).
 static int clusters_at_once(int blocks) {
-    static int known[64][4];
+    static int known[64][5];
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess) return 0;
-    const int which = blocks == 1 ? 0 : blocks == 2 ? 1 : blocks == 4 ? 2 : 3;
+    const int which = blocks == 1 ? 0 : blocks == 2 ? 1 : blocks == 4 ? 2 : blocks == 8 ? 3 : 4;
     int n = device < 64 ? __atomic_load_n(&known[device][which], __ATOMIC_RELAXED) : 0;
     if (n > 0) return n;
+    if (blocks > 8 && cudaFuncSetAttribute(attention_cross_tc_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) { cudaGetLastError(); return 0; }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(blocks * 148);
+    cfg.gridDim = dim3(blocks * 296);
     cfg.blockDim = dim3(XT_THREADS);
     cfg.dynamicSmemBytes = XT_SMEM;
     cudaLaunchAttribute attr[1];
@@ -635,22 +576,22 @@ static int clusters_at_once(int blocks) {
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, attention_cross_tc_kernel, &cfg) != cudaSuccess || n < 1) { cudaGetLastError(); n = 148 / blocks; }
-    if (blocks == 1 && n > 148) n = 148;
+    if (cudaOccupancyMaxActiveClusters(&n, attention_cross_tc_kernel, &cfg) != cudaSuccess || n < 1) { cudaGetLastError(); if (blocks > 8) return 0; n = 296 / blocks; }
     if (device < 64) __atomic_store_n(&known[device][which], n, __ATOMIC_RELAXED);
     return n;
 }
 
-// Over how many blocks of a cluster a tile pair's keys are cut: the fewest rounds over the SMs, a round counted in cycles: a block's way in and out, a cluster's meeting,
-// and the blocks of 64 keys (both halves on the same rows: half as long each).
-static int choose_chunks(long long pairs, int longest, bool one_tile) {
+// Over how many blocks of a cluster the keys of a tile are cut: the fewest rounds over the SMs, a round counted in cycles: a block's way in and out, a cluster's
+// meeting, and the blocks of 64 keys.
+static int choose_chunks(long long jobs, int longest) {
     const int keys = (longest + XT_BN - 1) / XT_BN;
     int best = 1;
     long long least = 0;
     for (int c = 1; c <= XT_MAX_CLUSTER; c *= 2) {
         if (c > 1 && keys < 4 * c) break;
         const int room = clusters_at_once(c);
-        const long long rounds = (pairs + room - 1) / room, cost = rounds * (XT_COST_BLOCK + (c > 1 ? XT_COST_CLUSTER : 0) + (long long)((keys + c - 1) / c) * (one_tile ? XT_COST_SOLO : XT_COST_KEYS));
+        if (room < 1) break;
+        const long long rounds = (jobs + room - 1) / room, cost = rounds * (XT_COST_BLOCK + (c > 1 ? XT_COST_CLUSTER : 0) + (long long)((keys + c - 1) / c) * XT_COST_KEYS);
         if (c == 1 || cost < least) { best = c; least = cost; }
     }
     return best;
@@ -661,23 +602,23 @@ MB_API int mb_attention_cross_tc(const CrossCall* c, cudaStream_t s) {
     if (c->requests <= 0 || c->max_query <= 0) return 0;
     const long long cache_rows = c->cache_pages * c->K * c->page_size;
     if (!cross_call_fits(c) || c->d != D || c->dtype != MB_BF16 || c->page_size < 16 || c->page_size > 128 || c->H / c->K > XT_BM || cache_rows <= 0 || cache_rows > 0x7fffff00LL ||
-        (((uintptr_t)c->q | (uintptr_t)c->k_cache | (uintptr_t)c->v_cache | (uintptr_t)c->out) & 15) != 0 || c->q_stride % 8 != 0 || (c->chunks != 0 && !chunks_fit(c->chunks)) ||
+        (((uintptr_t)c->q | (uintptr_t)c->k_cache | (uintptr_t)c->v_cache | (uintptr_t)c->out) & 15) != 0 || c->q_stride % 8 != 0 || (c->chunks != 0 && (!chunks_fit(c->chunks) || clusters_at_once(c->chunks) < 1)) ||
         (long long)c->H * D * 2 * XT_BM > 0x7fffffffLL)
         return MB_ERR_BAD_SIZE;
     const int G = c->H / c->K, per_tile = XT_BM / G;
-    const long long pairs = (c->max_query + 2LL * per_tile - 1) / (2 * per_tile);
-    if (pairs * c->requests > 0x7fffffffLL) return MB_ERR_BAD_SIZE;
+    const long long tiles = (c->max_query + (long long)per_tile - 1) / per_tile;
+    if (tiles * c->requests > 0x7fffffffLL) return MB_ERR_BAD_SIZE;
     static LaunchSmem allowed;
     int rc = allowed.allow(attention_cross_tc_kernel, XT_SMEM);
     if (rc != 0) return rc;
-    // (requests of unlike lengths: no more pairs than their tokens fill, and one more each)
-    const long long filled = c->requests + (long long)c->tokens / (2 * per_tile), most = pairs * c->requests < filled ? pairs * c->requests : filled;
-    const int chunks = c->chunks != 0 ? c->chunks : choose_chunks(most * c->K, c->longest, c->max_query <= per_tile);
+    // (requests of unlike lengths: no more tiles than their tokens fill, and one more each)
+    const long long filled = c->requests + (long long)c->tokens / per_tile, most = tiles * c->requests < filled ? tiles * c->requests : filled;
+    const int chunks = c->chunks > 0 ? c->chunks : choose_chunks(most * c->K, c->longest);
     CUtensorMap mq, mk, mv;
     const int box_rows = c->page_size < XT_BN ? c->page_size : XT_BN;
     if ((rc = map_queries(&mq, c->q, c->q_stride, c->H, c->tokens, G, per_tile)) != 0) return rc;
     if ((rc = map_rows(&mk, c->k_cache, (uint64_t)cache_rows, (uint32_t)box_rows)) != 0) return rc;
     if ((rc = map_rows(&mv, c->v_cache, (uint64_t)cache_rows, (uint32_t)box_rows)) != 0) return rc;
-    const CrossTc arg = {cross_args(c), c->error_flag, c->first, (int)pairs, (int)cache_rows};
-    return launch_kernel(attention_cross_tc_kernel, dim3((unsigned)(c->requests * pairs), c->K, chunks), dim3(XT_THREADS), XT_SMEM, s, chunks, mq, mk, mv, arg);
+    const CrossTc arg = {cross_args(c), c->error_flag, c->first, (int)tiles, (int)cache_rows};
+    return launch_kernel(attention_cross_tc_kernel, dim3((unsigned)(c->requests * tiles), c->K, chunks), dim3(XT_THREADS), XT_SMEM, s, chunks, mq, mk, mv, arg);
 }

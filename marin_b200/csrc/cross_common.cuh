@@ -22,7 +22,7 @@ struct CrossArgs {
 };
 
 // What a call hands over, in one piece (a caller in Python pays for every argument): requests first .. first + requests - 1 of a step of `tokens` tokens, none
-// with more than max_query of them or a source longer than `longest`; chunks: how many blocks of a cluster share their keys (where the caller decides that).
+// with more than max_query of them or a source longer than `longest`; chunks: how many blocks of a cluster share their keys (0: the launcher decides).
 struct CrossCall {
     const void *q, *k_cache, *v_cache;
     void* out;
@@ -47,7 +47,7 @@ static inline bool cross_call_fits(const CrossCall* c) {
     return shift >= 0 && c->K > 0 && c->K <= 65535 && c->H > 0 && c->H % c->K == 0 && c->d > 0 && c->max_pages >= 0 && ((long long)c->max_pages << shift) <= 0x7fffff00LL &&
            c->scale > 0.0f;
 }
-static inline bool chunks_fit(int chunks) { return chunks == 1 || chunks == 2 || chunks == 4 || chunks == 8; }
+static inline bool chunks_fit(int chunks) { return chunks == 1 || chunks == 2 || chunks == 4 || chunks == 8 || chunks == 16; }
 
 // The positions token t of a request sees, cut to its source; (0, 0) where there are none.
 __device__ __forceinline__ int2 cross_range(const CrossArgs& a, int t, int len) {
@@ -105,6 +105,39 @@ __device__ __forceinline__ float cross_peer(uint32_t addr, int rank) {
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
     return v;
 }
+__device__ __forceinline__ float4 cross_peer4(uint32_t addr, int rank) {
+    uint32_t remote;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote) : "memory");
+    return v;
+}
+// One row's partial results of `blocks` (up to 32) blocks of a cluster: lane c asks block c for its maximum and sum; back come that block's factor (lane c) and the sum.
+// EXACT: exp2f, else the special-function unit's.
+template <bool EXACT>
+__device__ __forceinline__ float cross_factor(const float* m, const float* l, int blocks, float& sum) {
+    const int lane = threadIdx.x & 31;
+    const float mine = lane < blocks ? cross_peer((uint32_t)__cvta_generic_to_shared(m), lane) : -INFINITY;
+    const float part = lane < blocks ? cross_peer((uint32_t)__cvta_generic_to_shared(l), lane) : 0.0f;
+    const float top = warp_max(mine), x = mine - (top == -INFINITY ? 0.0f : top);
+    float f;
+    if (EXACT) f = exp2f(x);
+    else asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(f) : "f"(x));
+    sum = warp_sum(lane < blocks ? f * part : 0.0f);
+    return f;
+}
+// Four columns of the row (from `o` on) added over the blocks in rank order, each times its factor.
+__device__ __forceinline__ float4 cross_join4(const float* o, float factor, int blocks) {
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int c = 0; c < blocks; ++c) {
+        const float w = __shfl_sync(0xffffffffu, factor, c);
+        const float4 p = cross_peer4((uint32_t)__cvta_generic_to_shared(o), c);
+        v.x = fmaf(w, p.x, v.x); v.y = fmaf(w, p.y, v.y); v.z = fmaf(w, p.z, v.z); v.w = fmaf(w, p.w, v.w);
+    }
+    return v;
+}
+__device__ __forceinline__ bool not_finite(float4 v) { return !(fabsf(v.x) <= 3.0e38f && fabsf(v.y) <= 3.0e38f && fabsf(v.z) <= 3.0e38f && fabsf(v.w) <= 3.0e38f); }
 __device__ __forceinline__ void cross_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
