@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(XD_WARPS * 32) attention_cross_decode_kernel(C
 MB_API int mb_attention_cross_decode(const CrossCall* c, cudaStream_t s) {
     if (c->requests <= 0) return 0;
     if (!cross_call_fits(c) || c->d != D || c->dtype != MB_BF16 || c->page_size < XD_KEYS || c->H / c->K > 8 || ((uintptr_t)c->q & 3) != 0 || ((uintptr_t)c->out & 7) != 0 || c->q_stride % 2 != 0 ||
-        (((uintptr_t)c->k_cache | (uintptr_t)c->v_cache) & 15) != 0 || !chunks_fit(c->chunks) || c->chunks > XD_MAX_CLUSTER)
+        (((uintptr_t)c->k_cache | (uintptr_t)c->v_cache) & 15) != 0 || !chunks_fit(c->chunks))
         return MB_ERR_BAD_SIZE;
     static LaunchSmem allowed;
     const int rc = allowed.allow(attention_cross_decode_kernel, XD_SMEM);

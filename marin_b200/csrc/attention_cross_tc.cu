@@ -3,19 +3,24 @@
 //
 // No mask depends on the order of tokens, so a tile's 128 rows are (token, query head of the group) pairs: 128 / G tokens of all heads that share a kv
 // head, one TMA box of [tokens][G][64 columns]; a portion of seven tokens fills as much of a tile as it can, and keys are fetched once for all of them.
-// A block takes two such tiles (A, B) over the same keys, in blocks of 128:
-//   S = Q K^T     tcgen05.mma 128 x 128 x d, operands in shared memory (TMA, 128-byte swizzle, K-major), S in 128 columns of tensor memory;
-//   P = 2^(S - m) two threads a row: 64 scores each by tcgen05.ld, maximum, exponentials in pairs, P as bfloat16 over the row's own scores (tcgen05.st).  The
+// A block works on one tile at a time, in blocks of 64 keys:
+//   S = Q K^T     tcgen05.mma 128 x 64 x d, operands in shared memory (TMA, 128-byte swizzle, K-major), S in one of two buffers in tensor memory;
+//   P = 2^(S - m) a thread a row: 64 scores by tcgen05.ld, maximum, exponentials in pairs, P as bfloat16 over the row's own scores (tcgen05.st).  The
 //                 maximum that O and the sum are scaled by follows the true one only when that has moved by more than 8 (2^8, harmless in float32);
 //   O += P V      tcgen05.mma with P from tensor memory, V as it lies in the cache ([key][d], an MN-major operand), O in d columns.
-// While the rows of A work, the tensor core has B's products and the other way round: P V of A and the next S of A, then the same for B.
-// Warps 0..7 are A's rows, 8..15 B's (two threads a row, 64 keys of a block each: a scheduler has two warps for every tile), 16 loads Q and K, 17 loads V, 18 and 19
-// issue A's and B's products.  Sums, maxima and O are float32; P is rounded to
-// bfloat16 as the products' operand (its error, 2^-9 of a weight, is that of the rounding of the result; the sum takes the weights before it).
+// With two buffers of scores the rows work on one while the other's P V and next S are made.  Two blocks an SM (256 columns of tensor memory and about 100 KB each):
+// one's barriers, first loads and last stores are time in which the other works.
+// Warps 0..3 are the rows, 4 loads Q and K, 5 loads V, 6 issues the products.  Sums, maxima and O are float32; P is rounded to
+// bfloat16 as the products' operand (its error, at most 2^-8 of a weight, is that of the rounding of the result; the sum takes the weights before it).
+// Measured on B200 (heads of 128, four prompts of 1,024 tokens of 32 heads over 4,096 positions, 275 GFLOP): 240 us (277 over
+// seconds, at the power limit's clock of 1.6 GHz).  What was tried: two tiles a block over the same
+// keys, one block an SM, with blocks of 128 keys (267 us) or 64 (262), with two threads a row (258 to 272), an issuer for both (274): slower, although a
+// key then comes for twice as many rows; blocks that stay and take tile after tile, loads ahead into the next (265); the special-function unit's exponentials by a
+// polynomial for a part of the scores (no gain).
 //
 // Few rows: the blocks of keys are cut over a cluster of up to eight blocks, which add their partial O in shared memory in rank order.
-// What is not there: keys past the source are masked; values past it are zeros (0 * NaN is NaN): whole pages by copies outside the tensor, the page that
-// ends inside by plain stores.  Waits are bounded and record a code in *error_flag.
+// What is not there: keys past the source are masked; values past it are zeros (0 * NaN is NaN): whole boxes by copies outside the tensor, the box that
+// the source ends in by plain stores.  Waits are bounded and record a code in *error_flag.
 #define MB_LIB "attention_cross_tc"
 #define MB_LIB_ID 43
 #include "tc_common.cuh"
@@ -50,15 +55,8 @@ static_assert(D % 64 == 0 || XT_BM * (D * 2 + 16) <= XT_TILE, "a tile's results 
 #define XT_THREADS 256                           // warps 0..3 the rows, 4 loads Q and K, 5 V, 6 issues the products
 static_assert(XT_BM * XT_OLD * 4 <= XT_TILE + 2 * XT_STAGES * XT_KV, "partial results fit the tile's memory");
 static_assert(2 * (XT_SMEM + 1024 + XT_BM * 20 + 512) <= 233472, "two blocks an SM");
-#define XT_MAX_CLUSTER 16                        // (more than 8 is a size the device may refuse)
-// cycles: a block's way in and out, a cluster's meeting, 64 keys (see choose_chunks)
-#define XT_COST_BLOCK 9000
-#define XT_COST_CLUSTER 4000
-#define XT_COST_KEYS 1400
-#ifndef XT_POLY
-#define XT_POLY 0                                // of eight pairs of scores, how many go by the polynomial
-#endif
-
+#define XT_MAX_CLUSTER 8
+#define XT_SMS 148
 struct CrossTc {
     CrossArgs a;
     int* error_flag;
@@ -74,30 +72,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
-}
-// 2^x of a pair without the special-function unit, for x in [-126, 126] (below: 2^-126): x = n + f with n the nearest whole number (1.5 * 2^23 added and taken
-// off again), 2^f by a cubic fitted on [-1/2, 1/2] for the least largest relative error, 7.5e-5 (a weight is rounded to bfloat16, 2e-3, next), n added to the exponent.
-__device__ __forceinline__ void exp2_pair_poly(uint64_t x, float& p0, float& p1) {
-    float x0, x1, n0, n1;
-    of_pair(x, x0, x1);
-    x = pair_of(max_nan(x0, -126.0f), max_nan(x1, -126.0f));
-    uint64_t magic, t, n, f, p;
-    magic = pair_of(12582912.0f, 12582912.0f);
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(t) : "l"(x), "l"(magic));
-    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(n) : "l"(t), "l"(magic));
-    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(f) : "l"(x), "l"(n));
-    p = fma_pair(pair_of(0.05517167f, 0.05517167f), f, pair_of(0.24261113f, 0.24261113f));
-    p = fma_pair(p, f, pair_of(0.69326097f, 0.69326097f));
-    p = fma_pair(p, f, pair_of(0.99992806f, 0.99992806f));
-    of_pair(p, p0, p1);
-    of_pair(t, n0, n1);
-    p0 = __int_as_float(__float_as_int(p0) + (__float_as_int(n0) << 23));
-    p1 = __int_as_float(__float_as_int(p1) + (__float_as_int(n1) << 23));
 }
 // 32 columns of this thread's lane; nothing of v may be used before tmem_ld_wait.
 __device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, float* v) {
@@ -184,7 +158,7 @@ __global__ void __launch_bounds__(XT_THREADS, 2) attention_cross_tc_kernel(const
                                                                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CrossTc arg) {
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* sQ = smem;                                             // [panel][128 rows][128 B]
-    uint8_t* sK = sQ + XT_TILE;                                 // [stage][panel][128 rows][128 B]
+    uint8_t* sK = sQ + XT_TILE;                                     // [stage][panel][64 rows][128 B]
     uint8_t* sV = sK + XT_STAGES * XT_KV;
     uint64_t* bars = (uint64_t*)(sV + XT_STAGES * XT_KV);
     uint64_t* q_full = bars;
@@ -200,7 +174,7 @@ __global__ void __launch_bounds__(XT_THREADS, 2) attention_cross_tc_kernel(const
     volatile int* abort = (volatile int*)(tmem_slot + 1);
     __shared__ float s_m[XT_BM], s_l[XT_BM];
     __shared__ int2 s_range[XT_BM];
-    __shared__ int s_to[XT_BM];                                 // where a row's result begins, from the block's first token on; -1: no row
+    __shared__ int s_to[XT_BM];                                     // where a row's result begins, from the block's first token on; -1: no row
     __shared__ int s_seen[2][4];                                    // [first, end) that each warp's rows see
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     PDL_ENTER_EARLY();
@@ -416,12 +390,8 @@ __global__ void __launch_bounds__(XT_THREADS, 2) attention_cross_tc_kernel(const
                 for (int j = 0; j < 16; ++j) {
                     const uint64_t x = fma_pair(pair_of(s[c * 32 + 2 * j], s[c * 32 + 2 * j + 1]), scale2, base2);
                     float p0, p1;
-                    if ((j & 7) >= 8 - XT_POLY) {
-                        exp2_pair_poly(x, p0, p1);
-                    } else {
-                        of_pair(x, p0, p1);
-                        p0 = xt_exp2(p0); p1 = xt_exp2(p1);
-                    }
+                    of_pair(x, p0, p1);
+                    p0 = xt_exp2(p0); p1 = xt_exp2(p1);
                     sum2[j & 1] = add_pair(sum2[j & 1], pair_of(p0, p1));
                     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(packed[j]) : "f"(p1), "f"(p0));
                 }
@@ -435,8 +405,6 @@ __global__ void __launch_bounds__(XT_THREADS, 2) attention_cross_tc_kernel(const
             of_pair(add_pair(sum2[0], sum2[1]), u0, u1);
             l_run = l_run * corr + (u0 + u1);
         }
-        // (the polynomial makes a large number of a NaN: no sum of weights of at most 2^8 comes near it)
-        if (!(l_run < 1.0e30f)) l_run = __int_as_float(0x7fc00000);
         if (nblk == 0) warp_wait(q_full, 0, abort, error_flag, 42);     // (nothing to do in this block of a cluster: what was asked for has to land all the same)
         if (ok && nblk > 0) ok = warp_wait(&o_done[(nblk - 1) & 1], ((nblk - 1) >> 1) & 1, abort, error_flag, 47);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -556,45 +524,13 @@ static int map_queries(CUtensorMap* map, const void* q, long long stride, int H,
     return rc == CUDA_SUCCESS ? 0 : 1000 + (int)rc;
 }
 
-// How many clusters of so many blocks (one an SM) the device holds at once, asked once a device: clusters of eight leave SMs without one where an SM group has
-// no eight left (B200: 14 or so of the 18 that the SMs would make).
-static int clusters_at_once(int blocks) {
-    static int known[64][5];
-    int device = 0;
-    if (cudaGetDevice(&device) != cudaSuccess) return 0;
-    const int which = blocks == 1 ? 0 : blocks == 2 ? 1 : blocks == 4 ? 2 : blocks == 8 ? 3 : 4;
-    int n = device < 64 ? __atomic_load_n(&known[device][which], __ATOMIC_RELAXED) : 0;
-    if (n > 0) return n;
-    if (blocks > 8 && cudaFuncSetAttribute(attention_cross_tc_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) { cudaGetLastError(); return 0; }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(blocks * 296);
-    cfg.blockDim = dim3(XT_THREADS);
-    cfg.dynamicSmemBytes = XT_SMEM;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = blocks;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, attention_cross_tc_kernel, &cfg) != cudaSuccess || n < 1) { cudaGetLastError(); if (blocks > 8) return 0; n = 296 / blocks; }
-    if (device < 64) __atomic_store_n(&known[device][which], n, __ATOMIC_RELAXED);
-    return n;
-}
-
-// Over how many blocks of a cluster the keys of a tile are cut: the fewest rounds over the SMs, a round counted in cycles: a block's way in and out, a cluster's
-// meeting, and the blocks of 64 keys.
-static int choose_chunks(long long jobs, int longest) {
+// Over how many blocks of a cluster the keys of a tile are cut: while there are fewer blocks than SMs, none with fewer than four blocks of keys.  (B200, heads of 128, 1, 2, 4
+// and 8 blocks a tile: 32 tiles over 2,048 positions 25, 22, 16 and 17 us; 16 over 4,096 54, 34, 22 and 18; 80 over 4,096 51, 40, 46 and 53; 192 over 2,048 36, 50, 56, 94.)
+static int choose_chunks(long long tiles, int longest) {
     const int keys = (longest + XT_BN - 1) / XT_BN;
-    int best = 1;
-    long long least = 0;
-    for (int c = 1; c <= XT_MAX_CLUSTER; c *= 2) {
-        if (c > 1 && keys < 4 * c) break;
-        const int room = clusters_at_once(c);
-        if (room < 1) break;
-        const long long rounds = (jobs + room - 1) / room, cost = rounds * (XT_COST_BLOCK + (c > 1 ? XT_COST_CLUSTER : 0) + (long long)((keys + c - 1) / c) * XT_COST_KEYS);
-        if (c == 1 || cost < least) { best = c; least = cost; }
-    }
-    return best;
+    int c = 1;
+    while (c < XT_MAX_CLUSTER && tiles * c * 2 <= XT_SMS + XT_SMS / 12 && keys >= 8 * c) c *= 2;
+    return c;
 }
 
 // Pages of 16 to 128 positions; q, caches and out at 16 bytes, q_stride in whole 16-byte steps.
@@ -602,7 +538,7 @@ MB_API int mb_attention_cross_tc(const CrossCall* c, cudaStream_t s) {
     if (c->requests <= 0 || c->max_query <= 0) return 0;
     const long long cache_rows = c->cache_pages * c->K * c->page_size;
     if (!cross_call_fits(c) || c->d != D || c->dtype != MB_BF16 || c->page_size < 16 || c->page_size > 128 || c->H / c->K > XT_BM || cache_rows <= 0 || cache_rows > 0x7fffff00LL ||
-        (((uintptr_t)c->q | (uintptr_t)c->k_cache | (uintptr_t)c->v_cache | (uintptr_t)c->out) & 15) != 0 || c->q_stride % 8 != 0 || (c->chunks != 0 && (!chunks_fit(c->chunks) || clusters_at_once(c->chunks) < 1)) ||
+        (((uintptr_t)c->q | (uintptr_t)c->k_cache | (uintptr_t)c->v_cache | (uintptr_t)c->out) & 15) != 0 || c->q_stride % 8 != 0 || (c->chunks != 0 && !chunks_fit(c->chunks)) ||
         (long long)c->H * D * 2 * XT_BM > 0x7fffffffLL)
         return MB_ERR_BAD_SIZE;
     const int G = c->H / c->K, per_tile = XT_BM / G;

@@ -47,7 +47,7 @@ static inline bool cross_call_fits(const CrossCall* c) {
     return shift >= 0 && c->K > 0 && c->K <= 65535 && c->H > 0 && c->H % c->K == 0 && c->d > 0 && c->max_pages >= 0 && ((long long)c->max_pages << shift) <= 0x7fffff00LL &&
            c->scale > 0.0f;
 }
-static inline bool chunks_fit(int chunks) { return chunks == 1 || chunks == 2 || chunks == 4 || chunks == 8 || chunks == 16; }
+static inline bool chunks_fit(int chunks) { return chunks == 1 || chunks == 2 || chunks == 4 || chunks == 8; }
 
 // The positions token t of a request sees, cut to its source; (0, 0) where there are none.
 __device__ __forceinline__ int2 cross_range(const CrossArgs& a, int t, int len) {
