@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(XT_THREADS, 2) attention_cross_tc_kernel(const
         }
         if (ok) {
             uint4* stage = reinterpret_cast<uint4*>(sQ);            // (the queries': the products are done)
-            const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
+            const float inv = 1.0f / l_run;
             const bool sees = range.y > range.x;
             bool odd = false;
 #pragma unroll
@@ -486,8 +486,8 @@ __global__ void __launch_bounds__(XT_THREADS, 2) attention_cross_tc_kernel(const
             const float factor = cross_factor<false>(&s_m[done], &s_l[done], cluster, sum);
             float4 v = cross_join4(sO + (size_t)done * XT_OLD + min(4 * lane, D - 4), factor, cluster);
             const int2 rg = s_range[done];
-            const float inv = rg.y > rg.x && sum != 0.0f ? 1.0f / sum : 0.0f;
-            v = inv == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+            const float inv = 1.0f / sum;
+            v = rg.y > rg.x ? make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (4 * lane < D) {
                 uint2 w;
                 asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w.x) : "f"(v.y), "f"(v.x));

@@ -93,7 +93,7 @@ __device__ __noinline__ void cross_row_alone(const CrossArgs& a, int t, int head
                 if (c < a.d) acc = fmaf(pj, to_f32(cross_row<T>(a, a.v_cache, table, kh, key0 + j)[c]), acc);
             }
         }
-        if (c < a.d) out[c] = from_f32<T>(l == 0.0f ? 0.0f : acc / l);
+        if (c < a.d) out[c] = from_f32<T>(range.y > range.x ? acc / l : 0.0f);
     }
 }
 

@@ -2926,7 +2926,7 @@ def qk_norm_axes_write(rows: torch.Tensor, q_out: Optional[torch.Tensor], q_weig
 
 
 #: most requests of one ``page_step`` (the running sums over them lie in a block's shared memory)
-PAGE_STEP_REQUESTS = 16384
+PAGE_STEP_REQUESTS = 8192
 
 
 def page_step(before: torch.Tensor, after: torch.Tensor, table: torch.Tensor, free: torch.Tensor, count: torch.Tensor, page_size: int, left: torch.Tensor,

@@ -228,6 +228,35 @@ def test_cross_twice_and_from_a_graph(ops, dtype):
     torch.testing.assert_close(a.out.double(), a.want(), rtol=0, atol=4e-6 if dtype == torch.float32 else 2 * 4.6 * 2.0 ** -8)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_cross_infinite_scores(ops, dtype):
+    """What softmax makes of infinities: keys that score minus infinity have no weight; where all of them do, or one scores plus infinity, the result is NaN."""
+    case = Case(dtype, 8, 2, 64, 16, [1, 20], [200, 200], seed=8)
+    case.q[:, :] = 1.0
+    for r in range(2):
+        for j in range(0, 200, 3):
+            case.k[int(case.table[r, j // 16]), :, j % 16] = float("-inf")
+        case.keys[r][::3] = float("-inf")
+    torch.testing.assert_close(case.run(ops).double(), case.want(), rtol=0, atol=4e-6 if dtype == torch.float32 else 2 * 4.5 * 2.0 ** -8)
+    for r in range(2):
+        for page in case.table[r, :13].tolist():
+            case.k[page] = float("-inf")
+    assert torch.isnan(case.run(ops)).all()
+    for r in range(2):
+        case.k[int(case.table[r, 3]), :, 5] = float("inf")
+    assert torch.isnan(case.run(ops)).all()
+
+
+def test_cross_many_requests_and_long_batches(ops):
+    """More requests and tiles than places for blocks, single tokens ahead of portions of unlike lengths."""
+    rng = random.Random(3)
+    new = [1] * 150 + [rng.choice([2, 17, 33, 64, 65, 129]) for _ in range(40)]
+    src = [rng.choice([0, 1, 16, 63, 64, 65, 100, 333]) for _ in new]
+    Case(torch.bfloat16, 16, 4, 64, 16, new, src, seed=12).check(ops)
+    Case(torch.bfloat16, 5, 1, 128, 32, new, src, spread_spans(new, src, 4), seed=13).check(ops)
+    Case(torch.float32, 4, 2, 32, 16, new, src, spread_spans(new, src, 5), seed=14).check(ops)
+
+
 def test_cross_far_pages(ops):
     """Pages whose first element lies past 2^31 in the cache."""
     H, K, d, page = 4, 2, 128, 64
@@ -262,7 +291,7 @@ def axes_want(rows, qw, kw, eps, positions, axis_of, inv_freq, rotary, interleav
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("H,K,d,rotary,page", [(32, 8, 128, 128, 16), (40, 8, 128, 64, 32), (16, 16, 80, 80, 16), (14, 2, 96, 96, 64), (5, 1, 64, 64, 16), (3, 2, 256, 256, 16),
-                                               (4, 2, 40, 20, 4), (2, 1, 7, 6, 1), (6, 3, 512, 512, 16), (0, 4, 128, 128, 16), (1, 1, 24, 16, 16), (9, 3, 72, 48, 8), (64, 64, 32, 32, 16)])
+                                               (4, 2, 40, 20, 4), (2, 1, 7, 6, 1), (6, 3, 512, 512, 16), (0, 4, 128, 128, 16), (1, 1, 24, 16, 16), (9, 3, 72, 48, 8), (64, 64, 32, 32, 16), (1, 1, 256, 256, 16), (96, 8, 128, 128, 16)])
 def test_axes(ops, dtype, H, K, d, rotary, page):
     g = torch.Generator(device=DEV).manual_seed(d + H)
     for T, axes, interleaved, norm, wide, padded in ((1, 1, False, True, 0, 0), (9, 3, True, False, 8, 2), (70, 2, False, True, 16, 3), (33, 4, True, True, 5, 0), (12, 3, False, False, 0, 1)):
