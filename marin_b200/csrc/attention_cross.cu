@@ -3,13 +3,14 @@
 // A block takes 32 rows (16: single tokens) (token, head of the group) of one request and kv head and walks its keys in tiles of 64 with a running maximum and sum:
 //   S [rows x 64] = Q K^T  each thread 4 rows x 4 keys (single tokens 1 x 4), four elements of d a step from shared memory, in pairs;
 //   P = exp2(S - m)        rows over 16 lanes; P through shared memory;
-//   O [rows x d] += P V    each thread its rows x d / 16 columns, in registers, in pairs.
+//   O [rows x d] += P V    each thread its rows x d / 16 columns, in registers, in pairs; four keys a step.
 // A tile's values are asked for (cp.async) before S, the next tile's keys before the softmax, the places of their rows a tile earlier.
 // Work split: the source is cut into up to eight chunks by its own length alone, a cluster's blocks take one each and add their partial results in
 // shared memory in chunk order.  A row's arithmetic depends on its request's source and its range only, not on the batch, the portion or the tile: the same bits.
-// Bound by the latency of a tile's steps (three barriers, loads out of shared memory ahead of every sixteen multiply-adds, 3 to 4 warps a scheduler): five requests of 370
-// tokens in all, 16 heads of 64 over 2,908 positions 81 us (105 with tiles of 64 rows, page lookups in the loads and idle blocks that wait for their cluster); four of
-// 300 tokens, 32 heads of 128 over 600 positions 514 us, 23 TFLOP/s.
+// Bound by the latency of a tile's steps (three barriers, loads out of shared memory ahead of the multiply-adds, 4 to 8 warps a scheduler): five requests of 370
+// tokens in all, 16 heads of 64 over 2,908 positions 77 us (105 with tiles of 64 rows, page lookups in the loads and idle blocks that wait for their cluster; 82
+// with the weights read one by one, in pairs, instead of four at a time); four of 300 tokens, 32 heads of 128 over 600 positions 488 us, 24 TFLOP/s.
+// Blocks of 64 rows and 256 threads measured 76 and 520 us, 32 rows of 64 threads 88 and 676.
 #define MB_LIB "attention_cross"
 #define MB_LIB_ID 42
 #include "cross_common.cuh"
@@ -65,7 +66,7 @@ __global__ void __launch_bounds__(THREADS) attention_cross_kernel(const __grid_c
     float* sQ = cx_smem;                                            // [BM][LD]; later the partial results
     float* sK = sQ + BM * LD;
     float* sV = sK + CX_BN * LD;
-    uint64_t* sP = reinterpret_cast<uint64_t*>(sV + CX_BN * LD);    // [BM][CX_PSTRIDE]: every weight twice, as the products' pairs want it
+    float* sP = sV + CX_BN * LD;                                    // [BM][CX_PSTRIDE]
     __shared__ float s_m[BM], s_l[BM];
     __shared__ int s_lo[BM], s_hi[BM], s_first, s_last;
     __shared__ long long s_place[2][CX_BN];                         // where a tile's rows begin in the caches
@@ -182,7 +183,7 @@ __global__ void __launch_bounds__(THREADS) attention_cross_kernel(const __grid_c
             for (int j = 0; j < 4; ++j) {
                 const float pj = exp2f(s[i][j] - base);
                 sum += pj;
-                sP[(ty * RM + i) * CX_PSTRIDE + tx + 16 * j] = pair_of(pj, pj);
+                sP[(ty * RM + i) * CX_PSTRIDE + tx + 16 * j] = pj;
             }
 #pragma unroll
             for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
@@ -194,20 +195,22 @@ __global__ void __launch_bounds__(THREADS) attention_cross_kernel(const __grid_c
         cp_async_wait<1>();
         __syncthreads();
 #pragma unroll 2
-        for (int j = 0; j < CX_BN; j += 2) {
-            ulonglong2 pv[RM];
+        for (int j = 0; j < CX_BN; j += 4) {
+            float4 pv[RM];
 #pragma unroll
-            for (int i = 0; i < RM; ++i) pv[i] = *reinterpret_cast<const ulonglong2*>(sP + (ty * RM + i) * CX_PSTRIDE + j);
+            for (int i = 0; i < RM; ++i) pv[i] = *reinterpret_cast<const float4*>(sP + (ty * RM + i) * CX_PSTRIDE + j);
 #pragma unroll
-            for (int c = 0; c < DCH; ++c) {
+            for (int jj = 0; jj < 4; ++jj) {
+                uint64_t w[RM];
 #pragma unroll
-                for (int jj = 0; jj < 2; ++jj) {
+                for (int i = 0; i < RM; ++i) { const float p = jj == 0 ? pv[i].x : jj == 1 ? pv[i].y : jj == 2 ? pv[i].z : pv[i].w; w[i] = pair_of(p, p); }
+#pragma unroll
+                for (int c = 0; c < DCH; ++c) {
                     const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(sV + (j + jj) * LD + c * 64 + tx * 4);
 #pragma unroll
                     for (int i = 0; i < RM; ++i) {
-                        const uint64_t w = jj == 0 ? pv[i].x : pv[i].y;
-                        o[i][c][0] = fma_pair(w, v.x, o[i][c][0]);
-                        o[i][c][1] = fma_pair(w, v.y, o[i][c][1]);
+                        o[i][c][0] = fma_pair(w[i], v.x, o[i][c][0]);
+                        o[i][c][1] = fma_pair(w[i], v.y, o[i][c][1]);
                     }
                 }
             }
@@ -253,7 +256,7 @@ __global__ void __launch_bounds__(THREADS) attention_cross_kernel(const __grid_c
 template <typename T, int BM, int THREADS, int DCH>
 static int launch_cross(const CrossArgs& a, int first_request, int requests, int max_tiles, int clusters, int whole, int q_whole, cudaStream_t s) {
     constexpr int LD = DCH * 64 + 4;
-    const size_t smem = ((size_t)(BM + 2 * CX_BN) * LD + 2 * BM * CX_PSTRIDE) * sizeof(float);
+    const size_t smem = ((size_t)(BM + 2 * CX_BN) * LD + BM * CX_PSTRIDE) * sizeof(float);
     static LaunchSmem allowed;
     const int rc = allowed.allow(attention_cross_kernel<T, BM, THREADS, DCH>, smem);
     if (rc != 0) return rc;
