@@ -53,7 +53,8 @@ __global__ void __launch_bounds__(XD_WARPS * 32) attention_cross_decode_kernel(C
     a.block_table = pdl_fresh(a.block_table); a.lens = pdl_fresh(a.lens); a.cu_tokens = pdl_fresh(a.cu_tokens); a.spans = pdl_fresh(a.spans);
     const int r = first_request + blockIdx.x, kh = blockIdx.y, rank = blockIdx.z, cluster = gridDim.z, G = a.G;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int t = a.cu_tokens[r], len = max(0, min(a.lens[r], a.max_pages << a.page_shift));
+    const int t = a.cu_tokens[r], tokens = a.cu_tokens[r + 1] - t, len = max(0, min(a.lens[r], a.max_pages << a.page_shift));
+    if (tokens <= 0) return;                                        // (a padded request: all blocks of its clusters)
     const int2 range = cross_range(a, t, len);
     const int* table = a.block_table + (size_t)r * a.max_pages;
     // stages of 16 positions: the block's share, and of it every fourth for this warp
@@ -168,7 +169,8 @@ __global__ void __launch_bounds__(XD_WARPS * 32) attention_cross_decode_kernel(C
     {
         float* mine = reinterpret_cast<float*>(ring) + (lane >> 2) * D + 2 * (lane & 3);
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) *reinterpret_cast<float2*>(mine + c * 8) = make_float2(o[c][0] + o[c][2], o[c][1] + o[c][3]);
+        for (int c = 0; c < D / 8; ++c)                             // (a value that is infinite is so by the rounded weights' product: what they left may be 0 or negative)
+            *reinterpret_cast<float2*>(mine + c * 8) = make_float2(fabsf(o[c][0]) <= 3.0e38f ? o[c][0] + o[c][2] : o[c][0], fabsf(o[c][1]) <= 3.0e38f ? o[c][1] + o[c][3] : o[c][1]);
         if ((lane & 3) == 0) { w_m[warp][lane >> 2] = m; w_l[warp][lane >> 2] = l; }
     }
     __syncthreads();

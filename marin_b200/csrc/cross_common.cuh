@@ -41,11 +41,13 @@ static inline CrossArgs cross_args(const CrossCall* c) {
     return {c->q, c->k_cache, c->v_cache, c->out, c->block_table, c->lens, c->cu_tokens, c->spans, c->q_stride, c->max_pages, c->K, c->H / c->K, c->d,
             page_shift_of(c->page_size), c->scale};
 }
-// What every kernel asks of a call: sizes that fit, a power of two of positions a page.
+// What every kernel asks of a call: sizes that fit, a power of two of positions a page, results that do not lie over queries (which other blocks may still read).
 static inline bool cross_call_fits(const CrossCall* c) {
     const int shift = page_shift_of(c->page_size);
+    const long long bytes = c->dtype == MB_F32 ? 4 : 2;
     return shift >= 0 && c->K > 0 && c->K <= 65535 && c->H > 0 && c->H % c->K == 0 && c->d > 0 && c->max_pages >= 0 && ((long long)c->max_pages << shift) <= 0x7fffff00LL &&
-           c->scale > 0.0f;
+           c->scale > 0.0f && c->q_stride >= 0 &&
+           ((uintptr_t)c->q >= (uintptr_t)c->out + bytes * c->tokens * c->H * c->d || (uintptr_t)c->out >= (uintptr_t)c->q + bytes * ((c->tokens - 1) * c->q_stride + (long long)c->H * c->d));
 }
 static inline bool chunks_fit(int chunks) { return chunks == 1 || chunks == 2 || chunks == 4 || chunks == 8; }
 

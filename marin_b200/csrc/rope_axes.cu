@@ -338,6 +338,11 @@ MB_API int mb_heads_axes(const AxesCall* c, cudaStream_t s) {
         return MB_ERR_BAD_SIZE;
     const int heads_total = c->write_kv ? H + 2 * K : H;
     if (heads_total == 0) return 0;
+    // queries may be finished where they lie (a thread, or a warp, reads a head before it writes it), but not over other rows
+    const long long bytes = c->dtype == MB_F32 ? 4 : 2, row = (long long)H * d;
+    const uintptr_t rows = (uintptr_t)c->rows, q_out = (uintptr_t)c->q_out;
+    if (H > 0 && !(rows == q_out && c->row_stride == row) && rows < q_out + bytes * c->T * row && q_out < rows + bytes * ((c->T - 1) * c->row_stride + (long long)heads_total * d))
+        return MB_ERR_BAD_SIZE;
     const AxesRows p = {c->rows, const_cast<void*>(c->q_out), c->q_w, c->k_w, c->positions, c->axis_of, c->inv_freq, c->slots, c->write_kv ? const_cast<void*>(c->k_cache) : nullptr,
                         c->write_kv ? const_cast<void*>(c->v_cache) : nullptr, c->row_stride, c->cache_rows, c->eps, c->T, H, c->write_kv ? K : 0, d, c->axes, half, c->interleaved,
                         c->page_size, heads_total};

@@ -2879,7 +2879,8 @@ def qk_norm_axes_write(rows: torch.Tensor, q_out: Optional[torch.Tensor], q_weig
     weights ``[d]`` or None) and their pairs turned, pair ``i`` by ``positions[axis_of[i], t] * inv_freq[i]`` (``positions`` int32 ``[axes, T]``, ``axis_of`` int32 and
     ``inv_freq`` float32 ``[rotary_dim / 2]``; the angle in 64 bits); queries go to ``q_out`` ``[T, H * d]``, keys and values into the paged caches at ``slot_mapping``
     (negative: a padded token, nothing is stored).  ``rows`` ``[T, >= (H + 2 K) * d]`` may be columns of wider rows.  ``H = 0`` (``q_out`` None): an encoder's
-    keys and values alone; ``write_kv=False``: queries alone.  ``axis_of`` is held to the axes there are, places past the caches store nothing."""
+    keys and values alone; ``write_kv=False``: queries alone.  ``axis_of`` is held to the axes there are, places past the caches store nothing, and a slot is for one token of the call.
+    Queries alone may be finished where they lie (``q_out`` is ``rows``); ``q_out`` over any other rows is refused."""
     device = _on_current_device("qk_norm_axes_write", rows, q_out, q_weight, k_weight, positions, axis_of, inv_freq, slot_mapping, k_cache, v_cache)
     shape, dtype = rows.shape, rows.dtype
     wanted = (H + 2 * K if write_kv else H) * d
@@ -2908,6 +2909,8 @@ def qk_norm_axes_write(rows: torch.Tensor, q_out: Optional[torch.Tensor], q_weig
             raise KernelError("qk_norm_axes_write: positions of one axis at least")
     page_size = cache_rows = 0
     if write_kv:
+        if slot_mapping is None or k_cache is None or v_cache is None:
+            raise KernelError("qk_norm_axes_write: caches and slots are wanted where keys and values are written")
         _int32_on("qk_norm_axes_write", device, (slot_mapping,))
         cache = k_cache.shape
         if (k_cache.dtype is not dtype or v_cache.dtype is not dtype or len(cache) != 4 or cache != v_cache.shape or cache[1] != K or cache[3] != d
@@ -2936,7 +2939,7 @@ def page_step(before: torch.Tensor, after: torch.Tensor, table: torch.Tensor, fr
     laid on top of the free list (``free``, of which ``count[0]`` entries are filled) in the order of requests and positions, and pages are taken from its top.
     ``left`` ``[2]``: the pages then free, and 0.  The new tokens (``after - before`` of them, request by request) get ``cu_tokens`` ``[R + 1]`` and, in buffers of any room,
     ``req_index``, ``positions`` and ``slots``; the rest of the buffers is 0, 0 and -1 (a padded token).  Rows of ``table`` past what a request holds are
-    left as they were.  ``before``, ``after`` and ``count`` stay: the caller hands in ``after`` and ``left`` next time.
+    left as they were.  ``before``, ``after`` and ``count`` stay: the caller hands in ``after`` and ``left`` next time.  What is written must not lie over anything else here.
 
     All or nothing: where ``left[1]`` is 1 (the free list runs out), 2 (more new tokens than the buffers' room), 3 (a length is negative or longer than a row of the
     table) or 4 (``count`` or what is given back is more than ``free`` holds), no page moves, ``left[0]`` is ``count[0]`` and every token is a padded one."""
@@ -3011,7 +3014,7 @@ def attention_cross(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``p = softmax_j(scale * q[t, h] . k[j])`` over the source's positions, or with ``spans`` (int32 ``[T, 2]``) over those from ``spans[t, 0]`` up to but not
     including ``spans[t, 1]``; a token that sees nothing gets zeros.  Keys and values lie in pages ``[page, K, page_size, d]`` (a power of two of positions).  Of ``ctx`` it
     takes ``num_requests``, ``num_decode`` (the first requests, one token each), ``max_query_len`` and ``cu_tokens``; rows of ``q`` ``[T, H * d]`` past the last request's
-    are not read and those of ``out`` stay as they were.  ``q`` may be columns of wider rows."""
+    are not read and those of ``out`` stay as they were, and so does the row of a request without a token (a padded batch's).  ``q`` may be columns of wider rows; ``out`` must not lie over it."""
     table, lens, cu = source.block_table, source.lens, ctx.cu_tokens
     device = _on_current_device("attention_cross", q, k_cache, v_cache, out)
     _int32_on("attention_cross", device, (table, lens, cu) if spans is None else (table, lens, cu, spans))
@@ -3030,13 +3033,15 @@ def attention_cross(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise KernelError(f"attention_cross: block_table [{R}, pages], lens [{R}] and cu_tokens [{R + 1}] are wanted")
     if spans is not None and spans.shape != (T, 2):
         raise KernelError(f"attention_cross: spans are [{T}, 2]")
-    if not 0.0 < scale < float("inf"):
+    if not 1e-38 < scale < 1e38:
         raise KernelError(f"attention_cross: scale is a positive number, got {scale}")
     if T == 0 or R == 0:
         return
-    longest = max(0, int(source.longest))
+    if T == 1:
+        stride = H * d                                               # (of a single row it says nothing)
+    longest = max(0, min(int(source.longest), columns[1] * page_size, 0x7fffff00))
     at = (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr())
-    aligned = stride % 8 == 0 and (at[0] | at[1] | at[2] | at[3]) % 16 == 0
+    aligned = stride % 8 == 0 and stride >= H * d and (at[0] | at[1] | at[2] | at[3]) % 16 == 0
     where = (table.data_ptr(), lens.data_ptr(), cu.data_ptr(), _address(spans), _scratch_for(q.device).error.data_ptr(), stride, pages, scale, _code(q), columns[1])
     stream = _stream_of(device)
     for first, n, most, single in ((0, nd, 1, True), (nd, R - nd, ctx.max_query_len, False)):

@@ -247,6 +247,43 @@ def test_cross_infinite_scores(ops, dtype):
     assert torch.isnan(case.run(ops)).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,K,d", [(8, 2, 64), (32, 2, 128)])
+def test_cross_infinite_values(ops, dtype, H, K, d):
+    """A value that is infinite and seen makes its column infinite, and no other."""
+    case = Case(dtype, H, K, d, 16, [1, 1, 20], [300, 16, 300], seed=9)
+    for r in range(3):
+        case.v[int(case.table[r, 0]), :, 5, 3] = float("inf")
+        case.v[int(case.table[r, 0]), :, 7, 9] = float("-inf")
+        case.values[r][5, :, 3], case.values[r][7, :, 9] = float("inf"), float("-inf")
+    got, want = case.run(ops).double(), case.want()
+    assert torch.equal(got.isposinf(), want.isposinf()) and torch.equal(got.isneginf(), want.isneginf()) and want.isinf().sum() == 2 * 22 * H
+    whole = want.isfinite()
+    torch.testing.assert_close(got[whole], want[whole], rtol=0, atol=4e-6 if dtype == torch.float32 else 2 * 5.0 * 2.0 ** -8)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_cross_padded_batch(ops, dtype):
+    """Requests without a token among those of single tokens and behind them (what a captured step of a fixed size holds): the rows that others have, and those behind, are theirs."""
+    case = Case(dtype, 8, 2, 64, 16, [1, 1, 1], [100, 37, 64], seed=10, pad_rows=3)
+    want = case.want()
+    case.ctx.num_requests = case.ctx.num_decode = 6
+    case.ctx.cu_tokens = ints([0, 1, 2, 3, 3, 3, 3])
+    case.table, case.lens = torch.cat([case.table, case.table]), ints([100, 37, 64, 100, 37, 0])
+    got = case.run(ops).double()
+    assert torch.equal(got[3:], want[3:])
+    torch.testing.assert_close(got, want, rtol=0, atol=4e-6 if dtype == torch.float32 else 2 * 4.5 * 2.0 ** -8)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [[1, 1], [1], [9, 30]])
+def test_cross_one_row_for_all(ops, dtype, new):
+    """Queries that are one row in memory (a stride of nothing), and a single row with a stride that says nothing."""
+    case = Case(dtype, 8, 2, 64, 16, new, [100, 37][:len(new)], seed=16)
+    case.q = case.q[:1].expand(sum(new), -1) if len(new) > 1 else torch.as_strided(case.q, (1, 512), (3, 1))
+    case.check(ops)
+
+
 def test_cross_many_requests_and_long_batches(ops):
     """More requests and tiles than places for blocks, single tokens ahead of portions of unlike lengths."""
     rng = random.Random(3)
@@ -511,7 +548,7 @@ def test_refusals_on_the_device(ops):
     run = lambda **kw: ops.attention_cross(**{**dict(q=case.q, k_cache=case.k, v_cache=case.v, out=case.out, ctx=case.ctx, source=src, H=8, K=2, d=64, scale=0.1), **kw})  # noqa: E731
     for bad in (dict(q=case.q.float()), dict(k_cache=case.k.float()), dict(K=3), dict(d=32), dict(out=case.out[:, :8]), dict(spans=ints([[0, 1]])), dict(H=0), dict(q=case.q.cpu()),
                 dict(source=ops.Source(case.table.long(), case.lens, 30)), dict(source=ops.Source(case.table[:1], case.lens, 30)), dict(k_cache=case.k[:, :, :12], v_cache=case.v[:, :, :12]),
-                dict(q=case.q.half(), out=case.out.half(), k_cache=case.k.half(), v_cache=case.v.half())):
+                dict(q=case.q.half(), out=case.out.half(), k_cache=case.k.half(), v_cache=case.v.half()), dict(out=case.q), dict(scale=0.0), dict(scale=1e39), dict(scale=1e-50), dict(scale=float("nan"))):
         with pytest.raises(ops.KernelError):
             run(**bad)
     one = ints([0])
@@ -529,6 +566,32 @@ def test_refusals_on_the_device(ops):
                 inv_freq=torch.ones(32, device=DEV), rotary_dim=64, interleaved=False, slot_mapping=ints([0, 1, 2]), k_cache=k, v_cache=v, H=4, K=1, d=64)
     ops.qk_norm_axes_write(**good)
     for bad in (dict(rows=rows[:, :300]), dict(H=5), dict(rotary_dim=63), dict(rotary_dim=66), dict(positions=ints([0, 1, 2])), dict(axis_of=ints([0] * 31)), dict(inv_freq=torch.ones(32, device=DEV).double()),
-                dict(k_cache=k.float()), dict(slot_mapping=ints([0, 1])), dict(q_out=None), dict(q_weight=torch.ones(63, device=DEV)), dict(v_cache=v[:1]), dict(rows=rows.cpu()), dict(rows=rows.half())):
+                dict(k_cache=k.float()), dict(slot_mapping=ints([0, 1])), dict(q_out=None), dict(q_weight=torch.ones(63, device=DEV)), dict(v_cache=v[:1]), dict(rows=rows.cpu()), dict(rows=rows.half()),
+                dict(slot_mapping=None), dict(k_cache=None), dict(rows=torch.zeros(5, 384, device=DEV, dtype=torch.bfloat16)[:3], q_out=None, H=0, positions=ints([[0, 1]]))):
         with pytest.raises(ops.KernelError):
             ops.qk_norm_axes_write(**{**good, **bad})
+    whole = torch.zeros(4 * 384, device=DEV, dtype=torch.bfloat16)
+    with pytest.raises(ops.KernelError):
+        ops.qk_norm_axes_write(**{**good, "rows": whole[:3 * 384].view(3, 384), "q_out": whole[384:384 + 3 * 256].view(3, 256)})
+    assert ops.Source(case.table, case.lens, 1 << 40).longest == 1 << 40
+    run(source=ops.Source(case.table, case.lens, 1 << 40))            # (longer than the table's rows: no source is)
+    torch.testing.assert_close(case.out.double(), Case.want(_scaled(case, 0.1)), rtol=0, atol=2 * 4.5 * 2.0 ** -8)
+
+
+def _scaled(case, scale):
+    case.scale = scale
+    return case
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 20])
+def test_axes_where_they_lie(ops, dtype, d):
+    """Queries finished in place, as elsewhere."""
+    g = torch.Generator(device=DEV).manual_seed(2)
+    rows = torch.randn(700, 4 * d, generator=g, device=DEV).to(dtype)
+    out, positions = torch.empty_like(rows), torch.arange(1400, device=DEV, dtype=torch.int32).view(2, 700)
+    run = lambda to: ops.qk_norm_axes_write(rows, to, torch.ones(d, device=DEV), None, 1e-6, positions, ints([0, 1] * (d // 4)), torch.ones(d // 2, device=DEV), d, False, None, None, None,  # noqa: E731
+                                            4, 0, d, write_kv=False)
+    run(out)
+    run(rows)
+    assert torch.equal(rows, out)
