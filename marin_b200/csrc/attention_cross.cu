@@ -60,7 +60,7 @@ __device__ __forceinline__ void cross_tile(float* dst, const CrossArgs& a, const
 }
 
 template <typename T, int BM, int THREADS, int DCH>
-__global__ void __launch_bounds__(THREADS) attention_cross_kernel(const __grid_constant__ CrossArgs arg, int first_request, int max_tiles, int whole, int q_whole) {
+__global__ void __launch_bounds__(THREADS) attention_cross_kernel(const __grid_constant__ CrossArgs arg, int first_request, int requests, int max_tiles, int whole, int q_whole) {
     constexpr int RM = BM * 16 / THREADS, LD = DCH * 64 + 4;
     extern __shared__ __align__(16) float cx_smem[];
     float* sQ = cx_smem;                                            // [BM][LD]; later the partial results
@@ -74,7 +74,8 @@ __global__ void __launch_bounds__(THREADS) attention_cross_kernel(const __grid_c
     CrossArgs a = arg;
     a.q = pdl_fresh((const char*)a.q); a.k_cache = pdl_fresh((const char*)a.k_cache); a.v_cache = pdl_fresh((const char*)a.v_cache);
     a.block_table = pdl_fresh(a.block_table); a.lens = pdl_fresh(a.lens); a.cu_tokens = pdl_fresh(a.cu_tokens); a.spans = pdl_fresh(a.spans);
-    const int r = first_request + blockIdx.x / max_tiles, tile = blockIdx.x % max_tiles, kh = blockIdx.y;
+    const int2 which = cross_tile_of(a, first_request, requests, a.G, BM, max_tiles, blockIdx.x);
+    const int r = which.x, tile = which.y, kh = blockIdx.y;
     const int rank = blockIdx.z, t0 = a.cu_tokens[r], rows = (a.cu_tokens[r + 1] - t0) * a.G, row0 = tile * BM;
     if (row0 >= rows) return;                                       // (all blocks of a cluster)
     const int len = max(0, min(a.lens[r], a.max_pages << a.page_shift));
@@ -254,14 +255,14 @@ __global__ void __launch_bounds__(THREADS) attention_cross_kernel(const __grid_c
 }
 
 template <typename T, int BM, int THREADS, int DCH>
-static int launch_cross(const CrossArgs& a, int first_request, int requests, int max_tiles, int clusters, int whole, int q_whole, cudaStream_t s) {
+static int launch_cross(const CrossArgs& a, int first_request, int requests, CrossGrid grid, int clusters, int whole, int q_whole, cudaStream_t s) {
     constexpr int LD = DCH * 64 + 4;
     const size_t smem = ((size_t)(BM + 2 * CX_BN) * LD + BM * CX_PSTRIDE) * sizeof(float);
     static LaunchSmem allowed;
     const int rc = allowed.allow(attention_cross_kernel<T, BM, THREADS, DCH>, smem);
     if (rc != 0) return rc;
-    return launch_kernel(attention_cross_kernel<T, BM, THREADS, DCH>, dim3((unsigned)(requests * max_tiles), a.K, clusters), dim3(THREADS), smem, s, clusters, a, first_request,
-                         max_tiles, whole, q_whole);
+    return launch_kernel(attention_cross_kernel<T, BM, THREADS, DCH>, dim3((unsigned)grid.blocks, a.K, clusters), dim3(THREADS), smem, s, clusters, a, first_request,
+                         requests, grid.max_tiles, whole, q_whole);
 }
 
 MB_API int mb_attention_cross(const CrossCall* c, cudaStream_t s) {
@@ -273,10 +274,10 @@ MB_API int mb_attention_cross(const CrossCall* c, cudaStream_t s) {
     // up to 16 rows (single tokens): tiles of 16, half of the multiply-adds that a tile of 32 would spend on rows that are not there
     const long long rows = (long long)c->max_query * a.G;
     const int bm = rows <= 16 ? 16 : 32;
-    const long long tiles = (rows + bm - 1) / bm;
-    if (tiles * c->requests > 0x7fffffffLL) return MB_ERR_BAD_SIZE;
+    const CrossGrid grid = cross_grid(c, a.G, bm);
+    if (grid.blocks > 0x7fffffffLL) return MB_ERR_BAD_SIZE;
     const int clusters = cross_chunks(c->longest), dch = (a.d + 63) / 64;
-#define CX_CASE(T, B, N, C) return launch_cross<T, B, N, C>(a, c->first, c->requests, (int)tiles, clusters, whole, q_whole, s)
+#define CX_CASE(T, B, N, C) return launch_cross<T, B, N, C>(a, c->first, c->requests, grid, clusters, whole, q_whole, s)
 #define CX_WIDTHS(T, B, N) switch (dch) { case 1: CX_CASE(T, B, N, 1); case 2: CX_CASE(T, B, N, 2); case 3: CX_CASE(T, B, N, 3); default: CX_CASE(T, B, N, 4); }
     if (c->dtype == MB_F32) { if (bm == 16) CX_WIDTHS(float, 16, 256) else CX_WIDTHS(float, 32, 128) }
     if (c->dtype == MB_BF16) { if (bm == 16) CX_WIDTHS(bf16, 16, 256) else CX_WIDTHS(bf16, 32, 128) }

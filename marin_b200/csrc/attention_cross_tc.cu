@@ -60,7 +60,7 @@ static_assert(2 * (XT_SMEM + 1024 + XT_BM * 20 + 512) <= 233472, "two blocks an 
 struct CrossTc {
     CrossArgs a;
     int* error_flag;
-    int first_request, max_tiles, cache_rows;
+    int first_request, requests, max_tiles, cache_rows;
 };
 
 __device__ __forceinline__ float xt_exp2(float x) {
@@ -182,8 +182,9 @@ __global__ void __launch_bounds__(XT_THREADS, 2) attention_cross_tc_kernel(const
     a.q = pdl_fresh((const char*)a.q); a.v_cache = pdl_fresh((const char*)a.v_cache); a.k_cache = pdl_fresh((const char*)a.k_cache);
     a.block_table = pdl_fresh(a.block_table); a.lens = pdl_fresh(a.lens); a.cu_tokens = pdl_fresh(a.cu_tokens); a.spans = pdl_fresh(a.spans);
     int* error_flag = arg.error_flag;
-    const int r = arg.first_request + blockIdx.x / arg.max_tiles, number = blockIdx.x % arg.max_tiles, kh = blockIdx.y;
-    const int rank = blockIdx.z, cluster = gridDim.z, G = a.G, per_tile = XT_BM / G;
+    const int rank = blockIdx.z, cluster = gridDim.z, kh = blockIdx.y, G = a.G, per_tile = XT_BM / G;
+    const int2 which = cross_tile_of(a, arg.first_request, arg.requests, 1, per_tile, arg.max_tiles, blockIdx.x);
+    const int r = which.x, number = which.y;
     const int tok0 = a.cu_tokens[r] + number * per_tile, left = a.cu_tokens[r + 1] - tok0;
     const int source = a.lens[r];
     if (left <= 0) return;                                          // (all blocks of a cluster)
@@ -542,19 +543,17 @@ MB_API int mb_attention_cross_tc(const CrossCall* c, cudaStream_t s) {
         (long long)c->H * D * 2 * XT_BM > 0x7fffffffLL)
         return MB_ERR_BAD_SIZE;
     const int G = c->H / c->K, per_tile = XT_BM / G;
-    const long long tiles = (c->max_query + (long long)per_tile - 1) / per_tile;
-    if (tiles * c->requests > 0x7fffffffLL) return MB_ERR_BAD_SIZE;
+    const CrossGrid grid = cross_grid(c, 1, per_tile);
+    if (grid.blocks > 0x7fffffffLL) return MB_ERR_BAD_SIZE;
     static LaunchSmem allowed;
     int rc = allowed.allow(attention_cross_tc_kernel, XT_SMEM);
     if (rc != 0) return rc;
-    // (requests of unlike lengths: no more tiles than their tokens fill, and one more each)
-    const long long filled = c->requests + (long long)c->tokens / per_tile, most = tiles * c->requests < filled ? tiles * c->requests : filled;
-    const int chunks = c->chunks > 0 ? c->chunks : choose_chunks(most * c->K, c->longest);
+    const int chunks = c->chunks > 0 ? c->chunks : choose_chunks(grid.blocks * c->K, c->longest);
     CUtensorMap mq, mk, mv;
     const int box_rows = c->page_size < XT_BN ? c->page_size : XT_BN;
     if ((rc = map_queries(&mq, c->q, c->q_stride, c->H, c->tokens, G, per_tile)) != 0) return rc;
     if ((rc = map_rows(&mk, c->k_cache, (uint64_t)cache_rows, (uint32_t)box_rows)) != 0) return rc;
     if ((rc = map_rows(&mv, c->v_cache, (uint64_t)cache_rows, (uint32_t)box_rows)) != 0) return rc;
-    const CrossTc arg = {cross_args(c), c->error_flag, c->first, (int)tiles, (int)cache_rows};
-    return launch_kernel(attention_cross_tc_kernel, dim3((unsigned)(c->requests * tiles), c->K, chunks), dim3(XT_THREADS), XT_SMEM, s, chunks, mq, mk, mv, arg);
+    const CrossTc arg = {cross_args(c), c->error_flag, c->first, c->requests, grid.max_tiles, (int)cache_rows};
+    return launch_kernel(attention_cross_tc_kernel, dim3((unsigned)grid.blocks, c->K, chunks), dim3(XT_THREADS), XT_SMEM, s, chunks, mq, mk, mv, arg);
 }

@@ -58,6 +58,33 @@ __device__ __forceinline__ int2 cross_range(const CrossArgs& a, int t, int len) 
     return hi > lo ? make_int2(lo, hi) : make_int2(0, 0);
 }
 
+// Which tile of which request block `x` of a launch takes.  Tiles of `size` rows; all requests have max_tiles of them (what the longest portion needs), or, with max_tiles = 0,
+// request r's begin at place floor(rows ahead of it / size) + r, which leaves each as many places as it needs and one at most over: there are rows / size + requests
+// places, where a batch of one long portion and many short ones would launch mostly empty blocks otherwise.  Found 32 requests at a time; all lanes of a warp call it.
+__device__ __forceinline__ int2 cross_tile_of(const CrossArgs& a, int first, int requests, int rows_a_token, int size, int max_tiles, int x) {
+    if (max_tiles > 0) return make_int2(first + x / max_tiles, x % max_tiles);
+    const int lane = threadIdx.x & 31, base = a.cu_tokens[first];
+    int lo = 0, n = requests, begins = 0;
+    do {
+        const int step = (n + 31) / 32, at = lo + lane * step;
+        const int place = lane * step < n ? (int)((long long)(a.cu_tokens[first + at] - base) * rows_a_token / size) + at : 0x7fffffff;
+        const int k = max(0, __popc(__ballot_sync(0xffffffffu, place <= x)) - 1);
+        begins = __shfl_sync(0xffffffffu, place, k);
+        lo += k * step;
+        n = min(step, n - k * step);
+    } while (n > 1);
+    return make_int2(first + lo, x - begins);
+}
+// The launch's blocks and max_tiles of it: by the longest portion where that leaves few blocks without rows (no search then), else by the rows there are.  (B200, bfloat16, 32
+// heads of 128 over 8, the longest portion's tiles against the search: 31 requests of 16 tokens and one of 2,048 over 1,024 positions 129 and 64 us, 199 of 2 and one of 2,048
+// over 500 646 and 192; in 32 bits, 16 heads of 64, 464 and 426, 656 and 569; portions of one length have the same blocks either way.)
+struct CrossGrid { long long blocks; int max_tiles; };
+static inline CrossGrid cross_grid(const CrossCall* c, int rows_a_token, int size) {
+    const long long tiles = ((long long)c->max_query * rows_a_token + size - 1) / size, padded = tiles * c->requests, filled = c->requests + (long long)c->tokens * rows_a_token / size;
+    if (padded <= filled + filled / 4) return {padded, (int)tiles};
+    return {filled, 0};
+}
+
 template <typename T>
 __device__ __forceinline__ const T* cross_row(const CrossArgs& a, const void* cache, const int* table, int kh, int key) {
     const size_t page = (size_t)table[key >> a.page_shift];

@@ -74,7 +74,7 @@ class Case:
         for r, n in enumerate(self.new):
             s = self.src[r]
             for h in range(H):
-                limit = torch.tensor(self.limits[first:first + n], device=DEV)
+                limit = torch.tensor(self.limits[first:first + n], device=DEV, dtype=torch.int64).view(-1, 2)
                 at = torch.arange(s, device=DEV)
                 seen = (at >= limit[:, :1]) & (at < limit[:, 1:])
                 scores = self.q[first:first + n, h * d:(h + 1) * d].double() @ self.keys[r][:, h // G].t() * self.scale
@@ -292,6 +292,17 @@ def test_cross_many_requests_and_long_batches(ops):
     Case(torch.bfloat16, 16, 4, 64, 16, new, src, seed=12).check(ops)
     Case(torch.bfloat16, 5, 1, 128, 32, new, src, spread_spans(new, src, 4), seed=13).check(ops)
     Case(torch.float32, 4, 2, 32, 16, new, src, spread_spans(new, src, 5), seed=14).check(ops)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_cross_one_long_portion_among_many(ops, dtype):
+    """Tiles found by the rows there are: more requests than a search step looks at, some without a token, the long portion first, in the middle and last."""
+    for at, n, seed in ((0, 40, 1), (517, 1100, 2), (32, 33, 3), (0, 1, 4)):
+        new = [(2, 0, 5, 33)[i % 4] for i in range(n)]
+        new[at] = 700
+        src = [(17, 64, 0, 65, 30)[i % 5] for i in range(n)]
+        src[at] = 130
+        Case(dtype, 4, 2, 16, 16, new, src, seed=seed, pad_rows=2).check(ops)
 
 
 def test_cross_far_pages(ops):
