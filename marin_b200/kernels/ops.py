@@ -2809,27 +2809,22 @@ def gla_jobs(dtype, d: int, dv: int, rank: int) -> dict:
 
 # ---- a decoder that reads an encoder's states: heads with positions of several axes, the states' pages, attention to them ----
 
-def _on_current_device(what: str, *tensors) -> int:
-    """The current device: launches go to its current stream, and tensors of another device (or of the host) are refused."""
-    here = None
+def _refuse_elsewhere(what: str, *tensors) -> None:
+    """Launches go to the current device's current stream: a tensor of another device (or of the host) is refused."""
     for t in tensors:
-        if t is not None:
-            d = t.get_device()
-            if here is None and d >= 0:
-                here = _current_device()
-            if d != here:
-                raise KernelError(f"{what}: marin_b200 kernels run on tensors of the current CUDA device; there is no CPU path: got one on {t.device}")
-    return here
+        if t.get_device() < 0 or t.get_device() != _current_device():
+            raise KernelError(f"{what}: marin_b200 kernels run on tensors of the current CUDA device; there is no CPU path: got one on {t.device}")
 
 
-def _int32_on(what: str, here: Optional[int], tensors) -> int:
+def _int32_on(what: str, here: Optional[int], tensors, _int32=torch.int32) -> int:
     """The same for tensors that hold contiguous 32-bit whole numbers."""
+    if here is None:
+        here = tensors[0].get_device()
+        if here < 0 or here != _current_device():
+            here = -2                                                # (no tensor's)
     for t in tensors:
-        d = t.get_device()
-        if d != here or d < 0 or t.dtype is not torch.int32 or not t.is_contiguous():
-            if here is not None or d < 0 or d != _current_device() or t.dtype is not torch.int32 or not t.is_contiguous():
-                raise KernelError(f"{what}: expects contiguous int32 tensors on the current CUDA device, got {t.dtype} on {t.device}")
-            here = d
+        if t.get_device() != here or t.dtype is not _int32 or not t.is_contiguous():
+            raise KernelError(f"{what}: expects contiguous int32 tensors on the current CUDA device, got {t.dtype} on {t.device}")
     return here
 
 
@@ -2838,21 +2833,18 @@ _PAGE_STEP, _HEADS_AXES, _CROSS = (struct.Struct(f) for f in ("10P5i", "10P2qf10
 _packed_entries: dict = {}
 
 
-def _packed_entry(name: str, load):
-    fn = _packed_entries.get(name)
+def _packed_entry(symbol: str, name: str, d: int = 0):
+    """Entry point `symbol` of library `name` (compiled for heads of `d` where that is not 0)."""
+    fn = _packed_entries.get((symbol, d))
     if fn is None:
-        fn = getattr(load(), name.split(" ")[0])
+        fn = getattr(_lib(name) if d == 0 else _cross_lib(name, d), symbol)
         fn.argtypes = [ctypes.c_char_p, _c_void_p]
-        _packed_entries[name] = fn
+        _packed_entries[symbol, d] = fn
     return fn
 
 
 def _stream_of(device: int):
     return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
-
-
-def _address(t: Optional[torch.Tensor]) -> int:
-    return t.data_ptr() if t is not None else 0
 
 
 def axis_sections(sections, spread: bool = False) -> list:
@@ -2881,7 +2873,12 @@ def qk_norm_axes_write(rows: torch.Tensor, q_out: Optional[torch.Tensor], q_weig
     (negative: a padded token, nothing is stored).  ``rows`` ``[T, >= (H + 2 K) * d]`` may be columns of wider rows.  ``H = 0`` (``q_out`` None): an encoder's
     keys and values alone; ``write_kv=False``: queries alone.  ``axis_of`` is held to the axes there are, places past the caches store nothing, and a slot is for one token of the call.
     Queries alone may be finished where they lie (``q_out`` is ``rows``); ``q_out`` over any other rows is refused."""
-    device = _on_current_device("qk_norm_axes_write", rows, q_out, q_weight, k_weight, positions, axis_of, inv_freq, slot_mapping, k_cache, v_cache)
+    device = rows.get_device()
+    if device < 0 or device != _current_device():
+        _refuse_elsewhere("qk_norm_axes_write", rows)
+    for t in (q_out, q_weight, k_weight, inv_freq, k_cache, v_cache):
+        if t is not None and t.get_device() != device:
+            _refuse_elsewhere("qk_norm_axes_write", t)
     shape, dtype = rows.shape, rows.dtype
     wanted = (H + 2 * K if write_kv else H) * d
     if len(shape) != 2 or shape[1] < wanted or H < 0 or K < 0 or wanted <= 0:
@@ -2922,9 +2919,14 @@ def qk_norm_axes_write(rows: torch.Tensor, q_out: Optional[torch.Tensor], q_weig
         return
     if launch_log is not None:
         _cost(2 * T * wanted * rows.element_size() + 4 * axes * T, 8.0 * T * wanted)
-    _check(_packed_entry("mb_heads_axes", lambda: _lib("mb_rope_axes"))(_HEADS_AXES.pack(
-        rows.data_ptr(), _address(q_out), _address(q_weight), _address(k_weight), _address(positions), _address(axis_of), _address(inv_freq), _address(slot_mapping),
-        _address(k_cache), _address(v_cache), row_stride, cache_rows, eps, _code(rows), axes, rotary_dim, int(interleaved), page_size, T, H, K, d, int(write_kv)),
+    code = _DTYPE_CODE.get(dtype)
+    if code is None:
+        _code(rows)
+    _check(_packed_entry("mb_heads_axes", "mb_rope_axes")(_HEADS_AXES.pack(
+        rows.data_ptr(), 0 if q_out is None else q_out.data_ptr(), 0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(),
+        0 if positions is None else positions.data_ptr(), 0 if axis_of is None else axis_of.data_ptr(), 0 if inv_freq is None else inv_freq.data_ptr(),
+        0 if slot_mapping is None else slot_mapping.data_ptr(), 0 if k_cache is None else k_cache.data_ptr(), 0 if v_cache is None else v_cache.data_ptr(),
+        row_stride, cache_rows, eps, code, axes, rotary_dim, interleaved, page_size, T, H, K, d, write_kv),
         _stream_of(device)), "qk_norm_axes_write")
 
 
@@ -2954,7 +2956,7 @@ def page_step(before: torch.Tensor, after: torch.Tensor, table: torch.Tensor, fr
         raise KernelError(f"page_step: page_size {page_size} is no power of two")
     if launch_log is not None:
         _cost(4 * (2 * R + R + 1 + 3 * room))
-    _check(_packed_entry("mb_page_step", lambda: _lib("mb_pages"))(_PAGE_STEP.pack(
+    _check(_packed_entry("mb_page_step", "mb_pages")(_PAGE_STEP.pack(
         before.data_ptr(), after.data_ptr(), table.data_ptr(), free.data_ptr(), count.data_ptr(), left.data_ptr(), cu_tokens.data_ptr(), req_index.data_ptr(), positions.data_ptr(),
         slots.data_ptr(), R, shape[1], free.numel(), page_size, room), _stream_of(device)), "page_step (tensors must not overlap)")
 
@@ -3016,7 +3018,9 @@ def attention_cross(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     takes ``num_requests``, ``num_decode`` (the first requests, one token each), ``max_query_len`` and ``cu_tokens``; rows of ``q`` ``[T, H * d]`` past the last request's
     are not read and those of ``out`` stay as they were, and so does the row of a request without a token (a padded batch's).  ``q`` may be columns of wider rows; ``out`` must not lie over it."""
     table, lens, cu = source.block_table, source.lens, ctx.cu_tokens
-    device = _on_current_device("attention_cross", q, k_cache, v_cache, out)
+    device = q.get_device()
+    if device < 0 or device != _current_device() or not device == k_cache.get_device() == v_cache.get_device() == out.get_device():
+        _refuse_elsewhere("attention_cross", q, k_cache, v_cache, out)
     _int32_on("attention_cross", device, (table, lens, cu) if spans is None else (table, lens, cu, spans))
     R, nd, dtype, shape, cache, columns = ctx.num_requests, ctx.num_decode, q.dtype, q.shape, k_cache.shape, table.shape
     if H <= 0 or K <= 0 or H % K or len(shape) != 2 or shape[1] != H * d or out.shape != shape or out.dtype is not dtype or not out.is_contiguous():
@@ -3042,18 +3046,21 @@ def attention_cross(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     longest = max(0, min(int(source.longest), columns[1] * page_size, 0x7fffff00))
     at = (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr())
     aligned = stride % 8 == 0 and stride >= H * d and (at[0] | at[1] | at[2] | at[3]) % 16 == 0
-    where = (table.data_ptr(), lens.data_ptr(), cu.data_ptr(), _address(spans), _scratch_for(q.device).error.data_ptr(), stride, pages, scale, _code(q), columns[1])
-    stream = _stream_of(device)
-    for first, n, most, single in ((0, nd, 1, True), (nd, R - nd, ctx.max_query_len, False)):
+    tables = (table.data_ptr(), lens.data_ptr(), cu.data_ptr(), 0 if spans is None else spans.data_ptr())
+    code, stream = _code(q), _stream_of(device)
+    for single in (True, False):
+        first, n, most = (0, nd, 1) if single else (nd, R - nd, ctx.max_query_len)
         if n <= 0:
             continue
+        error = 0
         if launch_log is not None:
             rows, size = (n if single else T - nd), q.element_size()
             _cost(size * (2 * rows * H * d + 2 * n * longest * K * d), 4.0 * rows * longest * H * d)
         if single and aligned and cross_decode_supported(dtype, H, K, d, page_size):
-            fn, chunks, what = _packed_entry(f"mb_attention_cross_decode {d}", lambda: _cross_lib("decode", d)), cross_decode_chunks(n * K, longest), "attention_cross (single tokens)"
+            fn, chunks, what = _packed_entry("mb_attention_cross_decode", "decode", d), cross_decode_chunks(n * K, longest), "attention_cross (single tokens)"
         elif aligned and cross_tc_supported(dtype, H, K, d, page_size) and 0 < pages * K * page_size < 0x7fffff00:
-            fn, chunks, what = _packed_entry(f"mb_attention_cross_tc {d}", lambda: _cross_lib("tc", d)), 0, "attention_cross (tensor cores)"
+            fn, chunks, what = _packed_entry("mb_attention_cross_tc", "tc", d), 0, "attention_cross (tensor cores)"
+            error = _scratch_for(q.device).error.data_ptr()
         else:
-            fn, chunks, what = _packed_entry("mb_attention_cross", lambda: _lib("mb_attention_cross")), 0, "attention_cross"
-        _check(fn(_CROSS.pack(*at, *where, first, n, most, T, chunks, longest, H, K, d, page_size), stream), what)
+            fn, chunks, what = _packed_entry("mb_attention_cross", "mb_attention_cross"), 0, "attention_cross"
+        _check(fn(_CROSS.pack(*at, *tables, error, stride, pages, scale, code, columns[1], first, n, most, T, chunks, longest, H, K, d, page_size), stream), what)
