@@ -74,8 +74,9 @@ __global__ void __launch_bounds__(THREADS) attention_cross_kernel(const __grid_c
     CrossArgs a = arg;
     a.q = pdl_fresh((const char*)a.q); a.k_cache = pdl_fresh((const char*)a.k_cache); a.v_cache = pdl_fresh((const char*)a.v_cache);
     a.block_table = pdl_fresh(a.block_table); a.lens = pdl_fresh(a.lens); a.cu_tokens = pdl_fresh(a.cu_tokens); a.spans = pdl_fresh(a.spans);
-    const int2 which = cross_tile_of(a, first_request, requests, a.G, BM, max_tiles, blockIdx.x);
-    const int r = which.x, tile = which.y, kh = blockIdx.y;
+    const int2 which = cross_tile_of(a, first_request, requests, a.G, BM, max_tiles, blockIdx.x / a.K);       // (a tile's heads side by side)
+    if (which.x < 0) return;
+    const int r = which.x, tile = which.y, kh = blockIdx.x % a.K;
     const int rank = blockIdx.z, t0 = a.cu_tokens[r], rows = (a.cu_tokens[r + 1] - t0) * a.G, row0 = tile * BM;
     if (row0 >= rows) return;                                       // (all blocks of a cluster)
     const int len = max(0, min(a.lens[r], a.max_pages << a.page_shift));
@@ -261,7 +262,7 @@ static int launch_cross(const CrossArgs& a, int first_request, int requests, Cro
     static LaunchSmem allowed;
     const int rc = allowed.allow(attention_cross_kernel<T, BM, THREADS, DCH>, smem);
     if (rc != 0) return rc;
-    return launch_kernel(attention_cross_kernel<T, BM, THREADS, DCH>, dim3((unsigned)grid.blocks, a.K, clusters), dim3(THREADS), smem, s, clusters, a, first_request,
+    return launch_kernel(attention_cross_kernel<T, BM, THREADS, DCH>, dim3((unsigned)grid.blocks * a.K, 1, clusters), dim3(THREADS), smem, s, clusters, a, first_request,
                          requests, grid.max_tiles, whole, q_whole);
 }
 
@@ -275,7 +276,7 @@ MB_API int mb_attention_cross(const CrossCall* c, cudaStream_t s) {
     const long long rows = (long long)c->max_query * a.G;
     const int bm = rows <= 16 ? 16 : 32;
     const CrossGrid grid = cross_grid(c, a.G, bm);
-    if (grid.blocks > 0x7fffffffLL) return MB_ERR_BAD_SIZE;
+    if (grid.blocks * a.K > 0x7fffffffLL) return MB_ERR_BAD_SIZE;
     const int clusters = cross_chunks(c->longest), dch = (a.d + 63) / 64;
 #define CX_CASE(T, B, N, C) return launch_cross<T, B, N, C>(a, c->first, c->requests, grid, clusters, whole, q_whole, s)
 #define CX_WIDTHS(T, B, N) switch (dch) { case 1: CX_CASE(T, B, N, 1); case 2: CX_CASE(T, B, N, 2); case 3: CX_CASE(T, B, N, 3); default: CX_CASE(T, B, N, 4); }

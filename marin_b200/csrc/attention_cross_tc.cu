@@ -182,8 +182,9 @@ __global__ void __launch_bounds__(XT_THREADS, 2) attention_cross_tc_kernel(const
     a.q = pdl_fresh((const char*)a.q); a.v_cache = pdl_fresh((const char*)a.v_cache); a.k_cache = pdl_fresh((const char*)a.k_cache);
     a.block_table = pdl_fresh(a.block_table); a.lens = pdl_fresh(a.lens); a.cu_tokens = pdl_fresh(a.cu_tokens); a.spans = pdl_fresh(a.spans);
     int* error_flag = arg.error_flag;
-    const int rank = blockIdx.z, cluster = gridDim.z, kh = blockIdx.y, G = a.G, per_tile = XT_BM / G;
-    const int2 which = cross_tile_of(a, arg.first_request, arg.requests, 1, per_tile, arg.max_tiles, blockIdx.x);
+    const int rank = blockIdx.z, cluster = gridDim.z, kh = blockIdx.x % a.K, G = a.G, per_tile = XT_BM / G;
+    const int2 which = cross_tile_of(a, arg.first_request, arg.requests, 1, per_tile, arg.max_tiles, blockIdx.x / a.K);    // (a tile's heads side by side)
+    if (which.x < 0) return;                                        // (all blocks of a cluster)
     const int r = which.x, number = which.y;
     const int tok0 = a.cu_tokens[r] + number * per_tile, left = a.cu_tokens[r + 1] - tok0;
     const int source = a.lens[r];
@@ -544,7 +545,7 @@ MB_API int mb_attention_cross_tc(const CrossCall* c, cudaStream_t s) {
         return MB_ERR_BAD_SIZE;
     const int G = c->H / c->K, per_tile = XT_BM / G;
     const CrossGrid grid = cross_grid(c, 1, per_tile);
-    if (grid.blocks > 0x7fffffffLL) return MB_ERR_BAD_SIZE;
+    if (grid.blocks * c->K > 0x7fffffffLL) return MB_ERR_BAD_SIZE;
     static LaunchSmem allowed;
     int rc = allowed.allow(attention_cross_tc_kernel, XT_SMEM);
     if (rc != 0) return rc;
@@ -555,5 +556,5 @@ MB_API int mb_attention_cross_tc(const CrossCall* c, cudaStream_t s) {
     if ((rc = map_rows(&mk, c->k_cache, (uint64_t)cache_rows, (uint32_t)box_rows)) != 0) return rc;
     if ((rc = map_rows(&mv, c->v_cache, (uint64_t)cache_rows, (uint32_t)box_rows)) != 0) return rc;
     const CrossTc arg = {cross_args(c), c->error_flag, c->first, c->requests, grid.max_tiles, (int)cache_rows};
-    return launch_kernel(attention_cross_tc_kernel, dim3((unsigned)grid.blocks, c->K, chunks), dim3(XT_THREADS), XT_SMEM, s, chunks, mq, mk, mv, arg);
+    return launch_kernel(attention_cross_tc_kernel, dim3((unsigned)grid.blocks * c->K, 1, chunks), dim3(XT_THREADS), XT_SMEM, s, chunks, mq, mk, mv, arg);
 }
