@@ -3002,10 +3002,10 @@ def _cross_lib(which: str, d: int):
 
 def cross_decode_chunks(pairs: int, longest: int) -> int:
     """Over how many blocks of a cluster (1, 2, 4 or 8) a single token's keys are cut, ``pairs`` requests times kv heads: more while there are fewer blocks than SMs, and once more for long sources that leave the SMs with few
-    blocks of unlike lengths.  (B200, heads of 128, 1 to 8 blocks each: 64 requests of 500 to 4,100 positions 103, 97, 105 and 143 us, of 577 all 31, 43, 60 and 92;
-    8 of 4,096 44, 29, 28 and 30; 2 of 2,000 to 4,096 36, 21, 13 and 10.)"""
+    blocks of unlike lengths; one where there are more pairs than places, which then take the longest first.  (B200, heads of 128, 1 to 8 blocks each: 64 requests of 500 to
+    4,100 positions 89, 96, 105 and 143 us, of 577 all 31, 43, 60 and 92; 8 of 4,096 44, 29, 28 and 30; 2 of 2,000 to 4,096 36, 21, 13 and 10.)"""
     chunks = 1
-    while chunks < 8 and ((pairs * chunks < SM_COUNT and chunks * 64 < longest) or (pairs * chunks <= 4 * SM_COUNT and chunks * 2048 <= longest)):
+    while chunks < 8 and ((pairs * chunks < SM_COUNT and chunks * 64 < longest) or (pairs <= 3 * SM_COUNT and pairs * chunks <= 4 * SM_COUNT and chunks * 2048 <= longest)):
         chunks *= 2
     return chunks
 

@@ -305,6 +305,21 @@ def test_cross_one_long_portion_among_many(ops, dtype):
         Case(dtype, 4, 2, 16, 16, new, src, seed=seed, pad_rows=2).check(ops)
 
 
+@pytest.mark.parametrize("K", [4, 64])
+@pytest.mark.parametrize("R", [127, 128, 129])
+def test_cross_many_single_tokens(ops, R, K):
+    """More single tokens than places for their blocks: every request once, sources of all lengths and of one, some of nothing; padded ones among them."""
+    rng = random.Random(R)
+    for src in ([rng.choice([0, 1, 17, 300, 301]) for _ in range(R)], [33] * R):
+        case = Case(torch.bfloat16, K, K, 16, 16, [1] * R, src, seed=R)
+        case.check(ops)
+    case.ctx.cu_tokens[R:] = R - 1                                    # the last has no token
+    case.out.fill_(7.0)
+    got, want = case.run(ops).double(), case.want()
+    assert (got[R - 1] == 7.0).all()
+    torch.testing.assert_close(got[:R - 1], want[:R - 1], rtol=0, atol=2 * 5.0 * 2.0 ** -8)
+
+
 def test_cross_far_pages(ops):
     """Pages whose first element lies past 2^31 in the cache."""
     H, K, d, page = 4, 2, 128, 64
