@@ -7,10 +7,11 @@
 // A tile's values are asked for (cp.async) before S, the next tile's keys before the softmax, the places of their rows a tile earlier.
 // Work split: the source is cut into up to eight chunks by its own length alone, a cluster's blocks take one each and add their partial results in
 // shared memory in chunk order.  A row's arithmetic depends on its request's source and its range only, not on the batch, the portion or the tile: the same bits.
-// Bound by the latency of a tile's steps (three barriers, loads out of shared memory ahead of the multiply-adds, 4 to 8 warps a scheduler): five requests of 370
-// tokens in all, 16 heads of 64 over 2,908 positions 77 us (105 with tiles of 64 rows, page lookups in the loads and idle blocks that wait for their cluster; 82
-// with the weights read one by one, in pairs, instead of four at a time); four of 300 tokens, 32 heads of 128 over 600 positions 488 us, 24 TFLOP/s.
-// Blocks of 64 rows and 256 threads measured 76 and 520 us, 32 rows of 64 threads 88 and 676.
+// Bound by the latency of a tile's steps (three barriers, loads out of shared memory ahead of the multiply-adds) at 2 to 3 blocks an SM: five requests of 370 tokens in all,
+// 16 heads of 64 over 2,908 positions 73 us (105 with tiles of 64 rows, page lookups in the loads and idle blocks that wait for their cluster; 82 with the weights read
+// one by one, in pairs, instead of four at a time); four of 300 tokens, 32 heads of 128 over 600 positions 480 us, 25 TFLOP/s, where the scores' products take 155, the
+// values' 100 and the copies 100 that the others do not cover.  Blocks of 64 rows and 256 threads measured 76 and 520 us, 32 rows of 64 threads 88 and 676; rows
+// copied whole by one thread each (cp.async.bulk) with two barriers a tile instead of four 74 and 465, and 116 for 110 with one request of 300 tokens: as good as the same.
 #define MB_LIB "attention_cross"
 #define MB_LIB_ID 42
 #include "cross_common.cuh"
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(THREADS) attention_cross_kernel(const __grid_c
         uint64_t s2[RM][4];
 #pragma unroll
         for (int i = 0; i < RM; ++i) s2[i][0] = s2[i][1] = s2[i][2] = s2[i][3] = 0;
-#pragma unroll 2
+#pragma unroll 4
         for (int x = 0; x < steps; ++x) {
             ulonglong2 kv[4], qv[RM];
 #pragma unroll
@@ -196,7 +197,7 @@ __global__ void __launch_bounds__(THREADS) attention_cross_kernel(const __grid_c
         }
         cp_async_wait<1>();
         __syncthreads();
-#pragma unroll 2
+#pragma unroll 4
         for (int j = 0; j < CX_BN; j += 4) {
             float4 pv[RM];
 #pragma unroll
