@@ -7,7 +7,7 @@
 // A tile's values are asked for (cp.async) before S, the next tile's keys before the softmax, the places of their rows a tile earlier.
 // Work split: the source is cut into up to eight chunks by its own length alone, a cluster's blocks take one each and add their partial results in
 // shared memory in chunk order.  A row's arithmetic depends on its request's source and its range only, not on the batch, the portion or the tile: the same bits.
-// Bound by the latency of a tile's steps (three barriers, loads out of shared memory ahead of the multiply-adds) at 2 to 3 blocks an SM: five requests of 370 tokens in all,
+// Bound by the latency of a tile's steps (four barriers, loads out of shared memory ahead of the multiply-adds) at 2 to 3 blocks an SM: five requests of 370 tokens in all,
 // 16 heads of 64 over 2,908 positions 73 us (105 with tiles of 64 rows, page lookups in the loads and idle blocks that wait for their cluster; 82 with the weights read
 // one by one, in pairs, instead of four at a time); four of 300 tokens, 32 heads of 128 over 600 positions 480 us, 25 TFLOP/s, where the scores' products take 155, the
 // values' 100 and the copies 100 that the others do not cover.  Blocks of 64 rows and 256 threads measured 76 and 520 us, 32 rows of 64 threads 88 and 676; rows

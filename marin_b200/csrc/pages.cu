@@ -7,8 +7,10 @@
 // request by bisection, its page in the block table or, if that page is one of this step's, in the stack; so there is no order between threads and no
 // atomic, and the results are the same bits in every run.  Reads and writes are disjoint: the free list is read below `count` and written from there on,
 // the block table is read where pages were held and written where they are new.
-// Every block makes the running sums itself (R additions of three numbers, the lengths in shared memory: a second launch or a wait between blocks would cost more).
-// Bound by latency: a launch, one round trip for the lengths, the sums' three rounds of shuffles, a bisection in shared memory, one round trip for a page.
+// Every block makes the running sums itself (R additions of three numbers, the lengths in shared memory: a second launch costs 2 to 3 us).
+// Bound by latency: a launch, one round trip for the lengths, the sums' three rounds of shuffles, a bisection in shared memory, one round trip for a page.  Measured on
+// B200, launches back to back: 8 requests 4.0 us, 256 with 24 prompts 4.6, 4,000 with 400 prompts and 100,000 new tokens 9.2 (12.0 with the lengths read again from memory by
+// every token and three counts one after the other); the call takes the host 7.
 #define MB_LIB "pages"
 #define MB_LIB_ID 40
 #include "common.cuh"

@@ -4,9 +4,12 @@
 // values copied; queries go to q_out, keys and values into the paged caches at the token's slot (a negative one: a padded token, nothing is stored).
 // The angle is a 64-bit product cut to a part of a turn: a 32-bit one is off by 2^-24 of the angle, 0.02 at position 300,000.  Cosine and sine are then
 // sincospif of a number within half a turn; norm and rotation run in 32 bits and are rounded once.
-// Bound by memory: every row is read and written once.  A block takes one token, all of its heads at once; a group of lanes takes a head, a lane two 16-byte
-// vectors that the rotation pairs (half-split: u and u + half / VEC) or two of the head's vectors (pairs side by side), so no value changes lanes; the
-// rows are asked for before the token's angles are worked out, once for all heads.
+// Bound by memory: every row is read and written once.  A group of lanes takes a head, a lane two 16-byte vectors that the rotation pairs (half-split: u and
+// u + half / VEC) or two of the head's vectors (pairs side by side), so no value changes lanes.  Two blocks an SM take equal runs of tokens, all heads at once: weights stay
+// in registers, three tokens' rows are on their way (a block a token had its threads wait for each token's rows and angles: 73 us at the first size below), and an angle is
+// worked out once for all heads, a thread an angle, tokens ahead of its use (the 64-bit product and sincospif are as many instructions as a head's whole norm and rotation).
+// Measured on B200: 8,007 tokens of 32 + 2 x 8 heads of 128, bfloat16, norm, three axes (197 MB): 37 us, 5.3 TB/s, 82 % of the copy rate (issue slots 64 % busy);
+// 2,501 tokens of 16 + 2 x 16 heads of 80, float32, pairs side by side (77 MB): 17 us, 4.5 TB/s; eight tokens 3 us, a launch and two trips to memory.
 #define MB_LIB "rope_axes"
 #define MB_LIB_ID 41
 #include "common.cuh"
