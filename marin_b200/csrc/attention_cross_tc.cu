@@ -417,48 +417,66 @@ __global__ void __launch_bounds__(XT_THREADS, 2) attention_cross_tc_kernel(const
         }
         if (ok) {
             uint4* stage = reinterpret_cast<uint4*>(sQ);            // (the queries': the products are done)
-            const float inv = 1.0f / l_run;
             const bool sees = range.y > range.x;
-            bool odd = false;
+            const float inv = 1.0f / l_run;
+            const uint64_t inv2 = pair_of(inv, inv);
+            uint64_t odd2 = 0;                                      // 0 times every result: NaN where one is not finite
 #pragma unroll
-            for (int c = 0; c < (D + 31) / 32; ++c) {               // 32 columns at a time (of the last ones what there is: tensor memory behind them is this block's own)
-                float o[32];
+            for (int c = 0; c < (D + 63) / 64; ++c) {               // 64 columns at a time (of the last ones what there is: tensor memory behind them is this block's own)
+                constexpr int MOST = D < 64 ? (D + 31) / 32 * 32 : 64;
+                float o[MOST];
                 if (nblk > 0) {
-                    tmem_ld32_async(o_col + c * 32, o);
+                    tmem_ld32_async(o_col + c * 64, o);
+                    if (MOST > 32) tmem_ld32_async(o_col + c * 64 + 32, o + MOST - 32);
                     tmem_ld_wait(o);
+                    if (MOST > 32) tmem_ld_wait(o + MOST - 32);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) o[j] = 0.0f;
+                    for (int j = 0; j < MOST; ++j) o[j] = 0.0f;
                 }
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    if (c * 32 + h * 8 >= D) continue;
+                for (int h = 0; h < MOST / 8; ++h) {
+                    if (c * 64 + h * 8 >= D) continue;
                     if (cluster > 1) {
-                        *reinterpret_cast<float4*>(sO + c * 32 + h * 8) = make_float4(o[8 * h], o[8 * h + 1], o[8 * h + 2], o[8 * h + 3]);
-                        *reinterpret_cast<float4*>(sO + c * 32 + h * 8 + 4) = make_float4(o[8 * h + 4], o[8 * h + 5], o[8 * h + 6], o[8 * h + 7]);
+                        *reinterpret_cast<float4*>(sO + c * 64 + h * 8) = make_float4(o[8 * h], o[8 * h + 1], o[8 * h + 2], o[8 * h + 3]);
+                        *reinterpret_cast<float4*>(sO + c * 64 + h * 8 + 4) = make_float4(o[8 * h + 4], o[8 * h + 5], o[8 * h + 6], o[8 * h + 7]);
                     } else {
                         uint32_t w[4];
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const float x = sees ? o[8 * h + 2 * j] * inv : 0.0f, y = sees ? o[8 * h + 2 * j + 1] * inv : 0.0f;
-                            odd |= !(fabsf(x) <= 3.0e38f) || !(fabsf(y) <= 3.0e38f);
+                            const uint64_t xy = mul_pair(pair_of(o[8 * h + 2 * j], o[8 * h + 2 * j + 1]), inv2);
+                            odd2 = fma_pair(xy, 0ull, odd2);
+                            float x, y;
+                            of_pair(xy, x, y);
                             asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[j]) : "f"(y), "f"(x));
                         }
-                        stage[XT_STAGED(tid, c * 4 + h)] = make_uint4(w[0], w[1], w[2], w[3]);
+                        stage[XT_STAGED(tid, c * 8 + h)] = sees ? make_uint4(w[0], w[1], w[2], w[3]) : make_uint4(0u, 0u, 0u, 0u);
                     }
                 }
             }
+            bool odd = false;
             if (cluster == 1) {
-                // a warp's rows out of shared memory, whole rows side by side (a thread its own row would touch 32 rows with every store)
+                // a warp's rows out of shared memory, whole rows side by side (a thread its own row would touch 32 rows with every store), eight pieces a lane at a time
                 __syncwarp();
-                constexpr int PIECES = D / 8, AT_ONCE = 32 / PIECES;
+                constexpr int PIECES = D / 8, AT_ONCE = 32 / PIECES, ROUNDS = (32 + AT_ONCE - 1) / AT_ONCE;
                 const int piece = lane % PIECES;
-#pragma unroll 4
-                for (int r0 = 0; r0 < 32; r0 += AT_ONCE) {
-                    const int rw = r0 + lane / PIECES, to = lane < AT_ONCE * PIECES && rw < 32 ? s_to[warp * 32 + rw] : -1;
-                    if (to >= 0) reinterpret_cast<uint4*>(out0 + to)[piece] = stage[XT_STAGED(warp * 32 + rw, piece)];
+#pragma unroll
+                for (int r0 = 0; r0 < ROUNDS; r0 += 8) {
+                    uint4 v[8];
+                    int to[8];
+#pragma unroll
+                    for (int e = 0; e < 8 && r0 + e < ROUNDS; ++e) {
+                        const int rw = (r0 + e) * AT_ONCE + lane / PIECES;
+                        to[e] = lane < AT_ONCE * PIECES && rw < 32 ? s_to[warp * 32 + rw] : -1;
+                        v[e] = stage[XT_STAGED(warp * 32 + min(rw, 31), piece)];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8 && r0 + e < ROUNDS; ++e)
+                        if (to[e] >= 0) reinterpret_cast<uint4*>(out0 + to[e])[piece] = v[e];
                 }
-                odd = odd && mine;
+                float z0, z1;
+                of_pair(odd2, z0, z1);
+                odd = mine && sees && z0 + z1 != 0.0f;
             }
             if (cluster > 1) { s_m[tid] = m_used; s_l[tid] = l_run; }
             if (a.spans != nullptr && cluster == 1) {
