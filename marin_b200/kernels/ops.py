@@ -3043,7 +3043,11 @@ def attention_cross(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         return
     if T == 1:
         stride = H * d                                               # (of a single row it says nothing)
-    longest = max(0, min(int(source.longest), columns[1] * page_size, 0x7fffff00))
+    longest, most = int(source.longest), columns[1] * page_size
+    if most > 0x7fffff00:
+        raise KernelError(f"attention_cross: {columns[1]} pages of {page_size} a request are more positions than 32 bits count")
+    if not 0 <= longest <= most:
+        longest = most if longest > 0 else 0
     at = (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr())
     aligned = stride % 8 == 0 and stride >= H * d and (at[0] | at[1] | at[2] | at[3]) % 16 == 0
     tables = (table.data_ptr(), lens.data_ptr(), cu.data_ptr(), 0 if spans is None else spans.data_ptr())
