@@ -7,11 +7,13 @@
 // A tile's values are asked for (cp.async) before S, the next tile's keys before the softmax, the places of their rows a tile earlier.
 // Work split: the source is cut into up to eight chunks by its own length alone, a cluster's blocks take one each and add their partial results in
 // shared memory in chunk order.  A row's arithmetic depends on its request's source and its range only, not on the batch, the portion or the tile: the same bits.
-// Bound by the latency of a tile's steps (four barriers, loads out of shared memory ahead of the multiply-adds) at 2 to 3 blocks an SM: five requests of 370 tokens in all,
-// 16 heads of 64 over 2,908 positions 73 us (105 with tiles of 64 rows, page lookups in the loads and idle blocks that wait for their cluster; 82 with the weights read
-// one by one, in pairs, instead of four at a time); four of 300 tokens, 32 heads of 128 over 600 positions 480 us, 25 TFLOP/s, where the scores' products take 155, the
-// values' 100 and the copies 100 that the others do not cover.  Blocks of 64 rows and 256 threads measured 76 and 520 us, 32 rows of 64 threads 88 and 676; rows
-// copied whole by one thread each (cp.async.bulk) with two barriers a tile instead of four 74 and 465, and 116 for 110 with one request of 300 tokens: as good as the same.
+// Bound by shared memory and by latency: for 16 multiply-add pairs twice, a thread asks for eight times 16 bytes, a warp's 512 bytes come at 128 a cycle, so the four warps of an SM
+// wait twice as long for them as their multiply-adds take; the rest are a tile's four barriers at 2 to 4 blocks an SM.  Five requests of 370 tokens in all, 16 heads of 64 over
+// 2,908 positions 73 us (105 with tiles of 64 rows, page lookups in the loads and idle blocks that wait for their cluster; 82 with the weights read one by one, in pairs,
+// instead of four at a time); four of 300 tokens, 32 heads of 128 over 600 positions 480 us, 25 TFLOP/s, where the scores' products take 155, the values' 100 and the copies 100
+// that the others do not cover.  Larger shares a thread (8 x 4, 8 x 8 sums) want registers that leave too few warps: 64 rows of 128 threads 78 and 567, of 256 threads 76 and 520,
+// of 64 threads 155 and 1,317; 32 rows of 64 threads 84 and 654; 2 x 8 sums (eight lanes a row) 90 and 568.  Rows copied whole by one thread each (cp.async.bulk) with two
+// barriers a tile instead of four 74 and 465, and 116 for 110 with one request of 300 tokens.
 #define MB_LIB "attention_cross"
 #define MB_LIB_ID 42
 #include "cross_common.cuh"
