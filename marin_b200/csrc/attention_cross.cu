@@ -1,7 +1,7 @@
 // Attention to an encoder's states in 32-bit arithmetic on the CUDA cores: float32 inputs, and bfloat16 ones of the layouts that the tensor-core
 // kernels do not take (the formula and the layout of rows: cross_common.cuh).
-// A block takes 32 rows (16: single tokens) (token, head of the group) of one request and kv head and walks its keys in tiles of 64 with a running maximum and sum:
-//   S [rows x 64] = Q K^T  each thread 4 rows x 4 keys (single tokens 1 x 4), four elements of d a step from shared memory, in pairs;
+// A block takes 32 rows (4, 8 or 16 where no request has more) (token, head of the group) of one request and kv head and walks its keys in tiles of 64 with a running maximum and sum:
+//   S [rows x 64] = Q K^T  each thread 4 rows x 4 keys (up to 16 rows: 1 x 4), four elements of d a step from shared memory, in pairs;
 //   P = exp2(S - m)        rows over 16 lanes; P through shared memory;
 //   O [rows x d] += P V    each thread its rows x d / 16 columns, in registers, in pairs; four keys a step.
 // A tile's values are asked for (cp.async) before S, the next tile's keys before the softmax, the places of their rows a tile earlier.
@@ -275,15 +275,18 @@ MB_API int mb_attention_cross(const CrossCall* c, cudaStream_t s) {
     const CrossArgs a = cross_args(c);
     const int whole = c->dtype == MB_F32 && a.d % 4 == 0 && (((uintptr_t)c->k_cache | (uintptr_t)c->v_cache) & 15) == 0;
     const int q_whole = c->dtype == MB_F32 && a.d % 4 == 0 && ((uintptr_t)c->q & 15) == 0 && c->q_stride % 4 == 0;
-    // up to 16 rows (single tokens): tiles of 16, half of the multiply-adds that a tile of 32 would spend on rows that are not there
+    // Few rows a request (single tokens): tiles of as few, for every row that is not there asks shared memory for keys and values all the same.  (Float32, tiles of 4 rows
+    // against tiles of 16: 8 single tokens over 2,000 positions, 16 heads of 64 48 and 92 us; 32 over 100 to 2,000 113 and 233; 32 over 600 positions,
+    // 32 heads of 128 over 8 81 and 117; 8 over 577 positions of the latter 40 and 39.)
     const long long rows = (long long)c->max_query * a.G;
-    const int bm = rows <= 16 ? 16 : 32;
+    const int bm = rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
     const CrossGrid grid = cross_grid(c, a.G, bm);
     if (grid.blocks * a.K > 0x7fffffffLL) return MB_ERR_BAD_SIZE;
     const int clusters = cross_chunks(c->longest), dch = (a.d + 63) / 64;
 #define CX_CASE(T, B, N, C) return launch_cross<T, B, N, C>(a, c->first, c->requests, grid, clusters, whole, q_whole, s)
 #define CX_WIDTHS(T, B, N) switch (dch) { case 1: CX_CASE(T, B, N, 1); case 2: CX_CASE(T, B, N, 2); case 3: CX_CASE(T, B, N, 3); default: CX_CASE(T, B, N, 4); }
-    if (c->dtype == MB_F32) { if (bm == 16) CX_WIDTHS(float, 16, 256) else CX_WIDTHS(float, 32, 128) }
-    if (c->dtype == MB_BF16) { if (bm == 16) CX_WIDTHS(bf16, 16, 256) else CX_WIDTHS(bf16, 32, 128) }
+#define CX_ROWS(T) { if (bm == 4) CX_WIDTHS(T, 4, 64) if (bm == 8) CX_WIDTHS(T, 8, 128) if (bm == 16) CX_WIDTHS(T, 16, 256) CX_WIDTHS(T, 32, 128) }
+    if (c->dtype == MB_F32) CX_ROWS(float)
+    if (c->dtype == MB_BF16) CX_ROWS(bf16)
     return MB_ERR_BAD_DTYPE;
 }
