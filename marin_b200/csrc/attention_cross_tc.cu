@@ -323,9 +323,9 @@ __global__ void __launch_bounds__(XT_THREADS, 2) attention_cross_tc_kernel(const
 #pragma unroll
                 for (int kk = 0; kk < XT_BN / 16; ++kk)
                     umma_bf16_tmem_a(tmem_o, tmem_s + (uint32_t)((i & 1) * XT_BN + kk * 8), vdesc + (uint32_t)(kk * (2048 >> 4)), idesc_pv, (i > 0 || kk > 0) ? 1u : 0u, elected);
-                if (more) scores(i + 2);                            // (S goes where P lies: the tensor core takes an issuer's products in their order)
                 umma_commit(&o_done[i & 1], elected);
                 umma_commit(&v_free[st], elected);
+                if (more) scores(i + 2);                            // (S goes where P lies: the tensor core takes an issuer's products in their order)
             }
             if (!ok && blocks > 0) {                                // (and what was issued has to end)
                 umma_commit(drained, elected);
@@ -349,8 +349,12 @@ __global__ void __launch_bounds__(XT_THREADS, 2) attention_cross_tc_kernel(const
             float s[XT_BN];
             tmem_ld32_async(s_col, s);
             tmem_ld32_async(s_col + 32, s + 32);
+            // (P V of the block before last is done, these scores came after it.  Its barrier's phase is seen all the same, each one by every warp: a wait for the next phase
+            // says nothing unless the one before is known to be over, and nothing orders the arrivals of two commits on two barriers.)
+            if (i >= 2) ok = warp_wait(&o_done[i & 1], ((i >> 1) - 1) & 1, abort, error_flag, 47);
             tmem_ld_wait(s);
             tmem_ld_wait(s + 32);
+            if (!ok) break;
             const int key0 = (block0 + i) * XT_BN, from = mask_from - key0, to = mask_to - key0;
             if (__any_sync(0xffffffffu, from > 0 || to < XT_BN)) {
 #pragma unroll
@@ -367,7 +371,7 @@ __global__ void __launch_bounds__(XT_THREADS, 2) attention_cross_tc_kernel(const
             const bool raise = m_true > m_used + 8.0f || (m_used == -INFINITY && m_true != -INFINITY);
             if (__any_sync(0xffffffffu, raise)) {
                 if (raise) { corr = xt_exp2(m_used - m_true); m_used = m_true; }
-                if (i > 0) {                                        // (P V of the blocks ahead has to be done; of the one before last it is, these scores came after it)
+                if (i > 0) {                                        // (P V of the blocks ahead has to be done)
                     ok = warp_wait(&o_done[(i - 1) & 1], ((i - 1) >> 1) & 1, abort, error_flag, 47);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
