@@ -62,8 +62,10 @@ __device__ __forceinline__ void cross_tile(float* dst, const CrossArgs& a, const
     cp_async_commit();
 }
 
+// Registers: four blocks of 256 threads an SM where shared memory has room for them (16 rows, heads up to 64; the rows worked out again would otherwise ask for more than the loop
+// does), and as many as there are for heads over 192, where it has room for one block (100 tokens of 8 heads of 256 over 500 positions, three requests: 108 us, 116 with 168).
 template <typename T, int BM, int THREADS, int DCH>
-__global__ void __launch_bounds__(THREADS) attention_cross_kernel(const __grid_constant__ CrossArgs arg, int first_request, int requests, int max_tiles, int whole, int q_whole) {
+__global__ void __launch_bounds__(THREADS, THREADS == 256 && DCH == 1 ? 4 : DCH == 4 ? 1 : 0) attention_cross_kernel(const __grid_constant__ CrossArgs arg, int first_request, int requests, int max_tiles, int whole, int q_whole) {
     constexpr int RM = BM * 16 / THREADS, LD = DCH * 64 + 4;
     extern __shared__ __align__(16) float cx_smem[];
     float* sQ = cx_smem;                                            // [BM][LD]; later the partial results
@@ -233,7 +235,10 @@ __global__ void __launch_bounds__(THREADS) attention_cross_kernel(const __grid_c
     }
     if (gridDim.z > 1) cross_cluster_sync(); else __syncthreads();
     // block `rank` finishes rows rank, rank + chunks, ...: a warp a row, the chunks in their order
+    constexpr int PIECES = DCH > 2 ? 2 : 1, AT_ONCE = BM == 32 ? 4 : 2;
     const int warp = tid >> 5, lane = tid & 31;
+    bool looked = false;
+    int2 odd_values = make_int2(0, 0);
     for (int row = rank + warp * chunks; row < BM; row += THREADS / 32 * chunks) {
         if (row0 + row >= rows) break;
         const bool sees = s_hi[row] > s_lo[row];
@@ -253,7 +258,17 @@ __global__ void __launch_bounds__(THREADS) attention_cross_kernel(const __grid_c
             if (c + 2 < a.d) out[c + 2] = from_f32<T>(v.z);
             if (c + 3 < a.d) out[c + 3] = from_f32<T>(v.w);
         }
-        if (a.spans != nullptr && __any_sync(0xffffffffu, odd)) { __syncwarp(); cross_row_alone<T>(arg, t, head, r, make_int2(s_lo[row], s_hi[row])); }
+        if (a.spans != nullptr && __any_sync(0xffffffffu, odd) && cross_sum_speaks(sum)) {
+            const int2 range = make_int2(s_lo[row], s_hi[row]);
+            if (cross_whole<T>(arg)) {
+                if (!looked) odd_values = cross_odd_values<T, PIECES, true>(arg, kh, r, first, last);
+                if (cross_not_its_own(odd_values, range)) { __syncwarp(); cross_row_alone<T, PIECES, AT_ONCE, true>(arg, t, head, r, range); }
+            } else {
+                if (!looked) odd_values = cross_odd_values<T, PIECES, false>(arg, kh, r, first, last);
+                if (cross_not_its_own(odd_values, range)) { __syncwarp(); cross_row_alone<T, PIECES, 1, false>(arg, t, head, r, range); }
+            }
+            looked = true;
+        }
     }
     if (gridDim.z > 1) cross_cluster_sync();                        // (a block's shared memory is read until here)
 }

@@ -480,17 +480,19 @@ __global__ void __launch_bounds__(XT_THREADS, 2) attention_cross_tc_kernel(const
                 }
                 float z0, z1;
                 of_pair(odd2, z0, z1);
-                odd = mine && sees && z0 + z1 != 0.0f;
+                odd = mine && sees && z0 + z1 != 0.0f && cross_sum_speaks(l_run);
             }
             if (cluster > 1) { s_m[tid] = m_used; s_l[tid] = l_run; }
             if (a.spans != nullptr && cluster == 1) {
                 unsigned which = __ballot_sync(0xffffffffu, odd);
+                const int2 odd_values = which != 0 ? cross_odd_values<bf16, 1, true>(arg.a, kh, r, first_block * XT_BN, min(len, (first_block + blocks_all) * XT_BN)) : make_int2(0, 0);
                 for (; which != 0; which &= which - 1) {
                     const int src = __ffs(which) - 1;
                     const int tok = __shfl_sync(0xffffffffu, my_tok, src), head = __shfl_sync(0xffffffffu, my_head, src);
                     const int2 rg = make_int2(__shfl_sync(0xffffffffu, range.x, src), __shfl_sync(0xffffffffu, range.y, src));
+                    if (!cross_not_its_own(odd_values, rg)) continue;
                     __syncwarp();
-                    cross_row_alone<bf16>(arg.a, tok0 + tok, head, r, rg);
+                    cross_row_alone<bf16, 1, 4, true>(arg.a, tok0 + tok, head, r, rg);
                 }
             }
         }
@@ -503,6 +505,8 @@ __global__ void __launch_bounds__(XT_THREADS, 2) attention_cross_tc_kernel(const
         cross_cluster_sync();
         // block `rank` finishes rows rank, rank + cluster, ...: a warp a row, four columns a lane
         const float* sO = (const float*)smem;
+        bool looked = false;
+        int2 odd_values = make_int2(0, 0);
         for (int done = rank + warp * cluster; done < XT_BM; done += (XT_THREADS / 32) * cluster) {
             const int to = s_to[done];
             if (to < 0) continue;
@@ -518,7 +522,10 @@ __global__ void __launch_bounds__(XT_THREADS, 2) attention_cross_tc_kernel(const
                 asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w.y) : "f"(v.w), "f"(v.z));
                 reinterpret_cast<uint2*>(out0 + to)[lane] = w;
             }
-            if (a.spans != nullptr && __any_sync(0xffffffffu, not_finite(v))) { __syncwarp(); cross_row_alone<bf16>(arg.a, tok0 + to / (a.K * G * D), to / D % (a.K * G), r, rg); }
+            if (a.spans != nullptr && __any_sync(0xffffffffu, not_finite(v)) && cross_sum_speaks(sum)) {
+                if (!looked) { looked = true; odd_values = cross_odd_values<bf16, 1, true>(arg.a, kh, r, first_block * XT_BN, min(len, (first_block + blocks_all) * XT_BN)); }
+                if (cross_not_its_own(odd_values, rg)) { __syncwarp(); cross_row_alone<bf16, 1, 4, true>(arg.a, tok0 + to / (a.K * G * D), to / D % (a.K * G), r, rg); }
+            }
         }
         cross_cluster_sync();                                       // (a block's shared memory is read until here)
     }

@@ -112,38 +112,132 @@ __device__ __forceinline__ const T* cross_row(const CrossArgs& a, const void* ca
     return (const T*)cache + (((page * a.K + kh) << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * a.d;
 }
 
-// One row's result from its own range alone, by one warp: where a result is not finite, a value that this row does not see may be what is not
-// (0 * infinity in a tile shared with rows that do see it).  All 32 lanes call it.
+// Four elements of a row of d from element c on, as they lie in memory (no branch between loads: many are on their way at once); what is past d is the row's last, to be left out by the
+// caller.  WHOLE: d is a multiple of four and rows begin where four elements can be read at once (cross_whole).
+template <typename T, bool WHOLE> struct CrossPiece;
+template <> struct CrossPiece<float, true> {
+    float4 raw;
+    __device__ __forceinline__ void load(const float* row, int c, int d) { raw = *reinterpret_cast<const float4*>(row + min(c, d - 4)); }
+    __device__ __forceinline__ float4 get() const { return raw; }
+};
+template <> struct CrossPiece<bf16, true> {
+    uint2 raw;
+    __device__ __forceinline__ void load(const bf16* row, int c, int d) { raw = *reinterpret_cast<const uint2*>(row + min(c, d - 4)); }
+    __device__ __forceinline__ float4 get() const { return make_float4(__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u), __uint_as_float(raw.y << 16), __uint_as_float(raw.y & 0xffff0000u)); }
+};
+template <typename T> struct CrossPiece<T, false> {
+    T raw[4];
+    __device__ __forceinline__ void load(const T* row, int c, int d) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) raw[e] = row[min(c + e, d - 1)];
+    }
+    __device__ __forceinline__ float4 get() const { return make_float4(to_f32(raw[0]), to_f32(raw[1]), to_f32(raw[2]), to_f32(raw[3])); }
+};
 template <typename T>
+__device__ __forceinline__ bool cross_whole(const CrossArgs& a) {
+    return a.d % 4 == 0 && a.q_stride % 4 == 0 && (((uintptr_t)a.q | (uintptr_t)a.k_cache | (uintptr_t)a.v_cache) & (4 * sizeof(T) - 1)) == 0;
+}
+__device__ __forceinline__ bool not_finite(float4 v) { return !(fabsf(v.x) <= 3.0e38f && fabsf(v.y) <= 3.0e38f && fabsf(v.z) <= 3.0e38f && fabsf(v.w) <= 3.0e38f); }
+
+// In a tile whose rows see different positions a value that is not finite reaches all of them (0 * infinity).  A row's result that is not finite is right all the same where
+//   * the row's own scores are not finite (its sum of weights, which are the row's alone, is NaN or 0: softmax gives NaN), or
+//   * every value of the tile's positions that is not finite is one that the row sees.
+// Else the row is worked out from its own range (cross_row_alone).  The call's other rows wait for that, so it is one pass over keys and values, a few positions at a time.
+// (B200, bfloat16, 32 heads of 128 over 8, 512 tokens over 2,000 positions, 0.05 ms: 0.2 ms where all rows see a value that is NaN, 3.3 where every second row has to be worked
+// out again, over 1,000 positions; 0.05 where a key is NaN.  64 tokens over 500 positions: 0.08 and 0.5; with a lane a position and every such row again 13.)
+__device__ __forceinline__ bool cross_sum_speaks(float sum) { return sum > 0.0f && sum < INFINITY; }       // (false where the sum itself says that the result is NaN)
+
+// The first and the last position of [from, to) with a value that is not finite, of one kv head; (0x7fffffff, -1): none.  P: pieces of four elements a lane (two for heads over
+// 128).  All 32 lanes of a warp call it, and get the same.
+template <typename T, int P, bool WHOLE>
+__device__ __noinline__ int2 cross_odd_values(const CrossArgs& a, int kh, int request, int from, int to) {
+    constexpr int U = 4;
+    const int lane = threadIdx.x & 31;
+    const int* table = a.block_table + (size_t)request * a.max_pages;
+    int first = 0x7fffffff, last = -1;
+    for (int key0 = from; key0 < to; key0 += U) {
+        CrossPiece<T, WHOLE> v[U][P];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int p = 0; p < P; ++p) v[u][p].load(cross_row<T>(a, a.v_cache, table, kh, min(key0 + u, to - 1)), 4 * lane + 128 * p, a.d);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            bool odd = not_finite(v[u][0].get());
+            if (P > 1) odd |= not_finite(v[u][P - 1].get());
+            if (odd) { first = min(first, min(key0 + u, to - 1)); last = max(last, min(key0 + u, to - 1)); }
+        }
+    }
+    return make_int2(__reduce_min_sync(0xffffffffu, first), __reduce_max_sync(0xffffffffu, last));
+}
+// Whether a row of this range has to be worked out again, `odd` being the tile's positions with values that are not finite.
+__device__ __forceinline__ bool cross_not_its_own(int2 odd, int2 range) { return !(odd.y >= 0 && odd.x >= range.x && odd.y < range.y); }
+
+// One row's result from its own range alone, by one warp, U positions at a time.  All 32 lanes call it.
+template <typename T, int P, int U, bool WHOLE>
 __device__ __noinline__ void cross_row_alone(const CrossArgs& a, int t, int head, int request, int2 range) {
     const int lane = threadIdx.x & 31, kh = head / a.G;
     const T* q = (const T*)a.q + (size_t)t * a.q_stride + (size_t)head * a.d;
     const int* table = a.block_table + (size_t)request * a.max_pages;
-    T* out = (T*)a.out + ((size_t)t * a.K * a.G + head) * a.d;
     const float sl2 = a.scale * 1.4426950408889634f;
-    auto score = [&](int key) {
-        const T* k = cross_row<T>(a, a.k_cache, table, kh, key);
-        float s = 0.0f;
-        for (int i = 0; i < a.d; ++i) s = fmaf(to_f32(q[i]), to_f32(k[i]), s);
-        return s * sl2;
-    };
-    float m = -INFINITY;
-    for (int key = range.x + lane; key < range.y; key += 32) { const float s = score(key); m = s != s ? s : fmaxf(m, s); if (m != m) break; }
-    const bool odd = __any_sync(0xffffffffu, m != m);
-    m = odd ? __int_as_float(0x7fc00000) : warp_max(m);
-    if (m == -INFINITY) m = 0.0f;
-    for (int c0 = 0; c0 < a.d; c0 += 32) {
-        const int c = c0 + lane;
-        float l = 0.0f, acc = 0.0f;
-        for (int key0 = range.x; key0 < range.y; key0 += 32) {
-            const float p = key0 + lane < range.y ? exp2f(score(key0 + lane) - m) : 0.0f;
-            for (int j = 0; j < 32 && key0 + j < range.y; ++j) {
-                const float pj = __shfl_sync(0xffffffffu, p, j);
-                l += pj;
-                if (c < a.d) acc = fmaf(pj, to_f32(cross_row<T>(a, a.v_cache, table, kh, key0 + j)[c]), acc);
+    float4 qp[P], acc[P];
+    bool in[P][4];                                                  // (elements past d: no part of a score)
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        CrossPiece<T, WHOLE> from;
+        from.load(q, 4 * lane + 128 * p, a.d);
+        qp[p] = from.get();
+        acc[p] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) in[p][e] = 4 * lane + 128 * p + (WHOLE ? 0 : e) < a.d;
+    }
+    float m = -INFINITY, l = 0.0f;
+    for (int key0 = range.x; key0 < range.y; key0 += U) {
+        CrossPiece<T, WHOLE> k[U][P], v[U][P];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {                               // (past the range: its last position, without a weight)
+            const int key = min(key0 + u, range.y - 1);
+            const T *keys = cross_row<T>(a, a.k_cache, table, kh, key), *values = cross_row<T>(a, a.v_cache, table, kh, key);
+#pragma unroll
+            for (int p = 0; p < P; ++p) { k[u][p].load(keys, 4 * lane + 128 * p, a.d); v[u][p].load(values, 4 * lane + 128 * p, a.d); }
+        }
+        float s[U], top = m;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            s[u] = 0.0f;
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                const float4 kp = k[u][p].get();
+                s[u] += (in[p][0] ? qp[p].x * kp.x : 0.0f) + (in[p][1] ? qp[p].y * kp.y : 0.0f) + ((in[p][2] ? qp[p].z * kp.z : 0.0f) + (in[p][3] ? qp[p].w * kp.w : 0.0f));
             }
         }
-        if (c < a.d) out[c] = from_f32<T>(range.y > range.x ? acc / l : 0.0f);
+#pragma unroll
+        for (int u = 0; u < U; ++u) { s[u] = warp_sum(s[u]) * sl2; top = fmaxf(top, s[u]); }
+        const float base = top == -INFINITY ? 0.0f : top, corr = exp2f(m - base);
+        m = top;
+        l *= corr;
+#pragma unroll
+        for (int p = 0; p < P; ++p) { acc[p].x *= corr; acc[p].y *= corr; acc[p].z *= corr; acc[p].w *= corr; }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (key0 + u >= range.y) continue;
+            const float w = exp2f(s[u] - base);
+            l += w;
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                const float4 vp = v[u][p].get();
+                acc[p].x = fmaf(w, vp.x, acc[p].x); acc[p].y = fmaf(w, vp.y, acc[p].y); acc[p].z = fmaf(w, vp.z, acc[p].z); acc[p].w = fmaf(w, vp.w, acc[p].w);
+            }
+        }
+    }
+    T* out = (T*)a.out + ((size_t)t * a.K * a.G + head) * a.d;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        const int c = 4 * lane + 128 * p;
+        const float of[4] = {acc[p].x, acc[p].y, acc[p].z, acc[p].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < a.d) out[c + e] = from_f32<T>(range.y > range.x ? of[e] / l : 0.0f);
     }
 }
 
@@ -187,7 +281,6 @@ __device__ __forceinline__ float4 cross_join4(const float* o, float factor, int 
     }
     return v;
 }
-__device__ __forceinline__ bool not_finite(float4 v) { return !(fabsf(v.x) <= 3.0e38f && fabsf(v.y) <= 3.0e38f && fabsf(v.z) <= 3.0e38f && fabsf(v.w) <= 3.0e38f); }
 __device__ __forceinline__ void cross_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }

@@ -48,3 +48,79 @@ def test_cross_scores_that_move_with_every_block(ops, dtype, step):
             case.out.zero_()
             assert torch.equal(case.run(ops), first)
     ops.check_device_errors()
+
+
+def put(case, r, j, value, columns=slice(None)):
+    """Position j of request r has this value (in the columns named), for every head."""
+    case.v[int(case.table[r, j // case.page]), :, j % case.page, columns] = value
+    case.values[r][j, :, columns] = value
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,K,d,page", [(8, 2, 64, 16), (32, 8, 128, 16), (4, 2, 20, 4), (3, 3, 7, 1), (4, 1, 200, 16), (2, 1, 256, 16), (40, 5, 48, 32)])
+@pytest.mark.parametrize("many", [1, 24])
+def test_cross_values_that_are_not_finite_concern_who_sees_them(ops, dtype, H, K, d, page, many):
+    """Infinities and NaN in values that some rows of a tile see, or all of them, or none: the rows that see them have them (in their columns), the others are as if they were
+    not there.  Spans begin and end at the value's place and beside it; cut over a cluster and not."""
+    src, at = 300, [70, 71, 200]
+    edges = [(0, 300), (0, 70), (0, 71), (70, 71), (71, 72), (71, 200), (72, 200), (72, 201), (200, 201), (201, 300), (5, 5), (64, 128), (128, 192), (0, 1)]
+    new = [1, len(edges)] + [9] * many
+    spans = [(72, 200)] + edges + [edges[i % len(edges)] for i in range(9 * many)]
+    case = Case(dtype, H, K, d, page, new, [src] * len(new), spans, seed=d)
+    clean = [v.clone() for v in case.values]
+    for r in range(len(new)):
+        put(case, r, at[0], float("nan"), slice(0, d // 2))
+        put(case, r, at[1], float("inf"), slice(d // 2, d // 2 + 1))
+        put(case, r, at[2], float("-inf"), slice(d - 2, d))
+    got, want = case.run(ops).double().view(-1, H, d), torch.empty(sum(new), H, d, device=DEV, dtype=torch.float64)
+    row, odd = 0, case.values
+    case.values = clean
+    want[:] = case.want().view(-1, H, d)
+    for r, n in enumerate(new):
+        for lo, hi in spans[row:row + n]:
+            for j in at:                                             # (a weight is positive: what is seen is there)
+                if lo <= j < hi:
+                    seen = odd[r][j].repeat_interleave(H // K, 0)
+                    want[row] = torch.where(seen.isfinite(), want[row], want[row] + seen)
+            row += 1
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isposinf(), want.isposinf()) and torch.equal(got.isneginf(), want.isneginf())
+    finite = want.isfinite()
+    torch.testing.assert_close(got[finite], want[finite], rtol=0, atol=4e-6 if dtype == torch.float32 else 2 * most_of(clean) * 2.0 ** -8)
+    ops.check_device_errors()
+
+
+@pytest.mark.parametrize("dtype,new", [(torch.bfloat16, 512), (torch.float32, 64)])
+def test_cross_price_of_a_value_that_is_not_finite(ops, dtype, new):
+    """A value (or a key) that is not finite does not hold up the step: where every row sees it nothing is worked out again; where some rows do not, theirs are, in one pass.
+    Bounds: reading a tile's values once more is less work than the call itself (a factor of 30 for the small launches here); the rows' own pass over 1,000 positions
+    is 100 instructions or so a row and position in a warp, at 4 warps an SM and one instruction in four cycles 512 * 32 * 1000 * 100 * 4 / (148 * 4) cycles, below 10 ms."""
+    spans = [(0, 2000) if t % 2 else (0, 1000) for t in range(new)]
+    case = Case(dtype, 32, 8, 128, 16, [new], [2000], spans, seed=3)
+
+    def milliseconds():
+        case.run(ops)
+        best = float("inf")
+        for _ in range(5):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            begin.record()
+            case.run(ops)
+            end.record()
+            end.synchronize()
+            best = min(best, begin.elapsed_time(end))
+        return best
+
+    usual = milliseconds()
+    page, at = int(case.table[0, 500 // 16]), 500 % 16
+    case.v[page, :, at] = float("nan")                               # (all see it)
+    seen_by_all = milliseconds()
+    assert case.out.isnan().all()
+    case.v[page, :, at] = 0.5
+    case.k[page, :, at] = float("nan")
+    key = milliseconds()
+    assert case.out.isnan().all()
+    case.k[page, :, at] = 0.5
+    case.v[int(case.table[0, 1500 // 16]), :, 1500 % 16] = float("inf")
+    seen_by_half = milliseconds()
+    assert case.out[1::2].isposinf().all() and case.out[::2].isfinite().all()
+    print(f"{new} tokens: {usual:.3f} ms, a value that all see {seen_by_all:.3f}, a key {key:.3f}, a value that half of the rows see {seen_by_half:.3f}")
+    assert key <= 2 * usual + 0.2 and seen_by_all <= 30 * usual + 0.2 and seen_by_half <= 10.0
