@@ -2886,6 +2886,8 @@ def qk_norm_axes_write(rows: torch.Tensor, q_out: Optional[torch.Tensor], q_weig
     T, (row_stride, column_stride) = shape[0], rows.stride()
     if column_stride != 1:
         raise KernelError("qk_norm_axes_write: a row's elements have to lie side by side")
+    if T == 1:
+        row_stride = wanted                                          # (of a single row it says nothing)
     if H > 0 and (q_out is None or q_out.shape != (T, H * d) or q_out.dtype is not dtype or not q_out.is_contiguous()):
         raise KernelError(f"qk_norm_axes_write: q_out is a contiguous {dtype} tensor [{T}, {H * d}]")
     for w in (q_weight, k_weight):

@@ -4,7 +4,7 @@ with the same tolerances as in ``test_source_operators_gpu.py``.
 import pytest
 import torch
 
-from test_source_operators_gpu import DEV, DTYPES, Case
+from test_source_operators_gpu import DEV, DTYPES, Case, axes_want, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -17,6 +17,10 @@ def ops():
 
 def most_of(values):
     return max([float(v.abs().max()) for v in values if v.numel()] or [1.0])
+
+
+def axes_tolerance(dtype):
+    return dict(rtol=2.0 ** -21, atol=2.0 ** -19) if dtype == torch.float32 else dict(rtol=2.0 ** -8, atol=2.0 ** -17)
 
 
 def climbing(dtype, new, src, step):
@@ -124,3 +128,17 @@ def test_cross_price_of_a_value_that_is_not_finite(ops, dtype, new):
     assert case.out[1::2].isposinf().all() and case.out[::2].isfinite().all()
     print(f"{new} tokens: {usual:.3f} ms, a value that all see {seen_by_all:.3f}, a key {key:.3f}, a value that half of the rows see {seen_by_half:.3f}")
     assert key <= 2 * usual + 0.2 and seen_by_all <= 30 * usual + 0.2 and seen_by_half <= 10.0
+
+
+# ---- heads with positions of several axes ----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("stride", [3, 4 * 64 + 24])
+def test_axes_single_row_in_place(ops, dtype, stride):
+    """A single token's queries finished where they lie: the row's stride says nothing, whether it is cut out of a wider row or made up."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    rows = torch.as_strided(torch.randn(4 * 64 + 24, generator=g, device=DEV).to(dtype), (1, 4 * 64), (stride, 1))
+    weight, positions, axis_of, inv_freq = 1 + 0.2 * torch.randn(64, generator=g, device=DEV), ints([[70], [5]]), ints([0, 1] * 16), torch.rand(32, generator=g, device=DEV)
+    want, _, _ = axes_want(rows, weight, None, 1e-6, positions, axis_of, inv_freq, 64, False, 4, 0, 64)
+    ops.qk_norm_axes_write(rows, rows, weight, None, 1e-6, positions, axis_of, inv_freq, 64, False, None, None, None, 4, 0, 64, write_kv=False)
+    torch.testing.assert_close(rows.double(), want.reshape(1, -1), **axes_tolerance(dtype))
