@@ -1,10 +1,12 @@
 """The operators of a decoder that reads an encoder's states, on the paths that only longer or larger calls take; against the same definitions in 64 bits and
 with the same tolerances as in ``test_source_operators_gpu.py``.
 """
+import random
+
 import pytest
 import torch
 
-from test_source_operators_gpu import DEV, DTYPES, Case, axes_want, ints
+from test_source_operators_gpu import DEV, DTYPES, Case, axes_want, ints, spread_spans
 
 pytestmark = pytest.mark.gpu
 
@@ -128,6 +130,43 @@ def test_cross_price_of_a_value_that_is_not_finite(ops, dtype, new):
     assert case.out[1::2].isposinf().all() and case.out[::2].isfinite().all()
     print(f"{new} tokens: {usual:.3f} ms, a value that all see {seen_by_all:.3f}, a key {key:.3f}, a value that half of the rows see {seen_by_half:.3f}")
     assert key <= 2 * usual + 0.2 and seen_by_all <= 30 * usual + 0.2 and seen_by_half <= 10.0
+
+
+def places(case):
+    """How the blocks of the portions' launch find their tiles: "longest" (requests), "sources" (the longest first), or "rows" (a search), by the rule beside the kernels."""
+    nd, G, f32 = case.ctx.num_decode, case.H // case.K, case.q.dtype == torch.float32
+    requests, T = case.ctx.num_requests - nd, case.q.shape[0]
+    rows = case.ctx.max_query_len * G
+    a_token, size = (G, 4 if rows <= 4 else 8 if rows <= 8 else 16 if rows <= 16 else 32) if f32 else (1, 128 // G)
+    padded, filled = -(-case.ctx.max_query_len * a_token // size) * requests, requests + T * a_token // size
+    if 1 < requests <= 32 and min(padded, filled) * case.K > 296:
+        return "sources"
+    return "longest" if padded <= filled + filled // 4 else "rows"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("portions", [2, 7, 31, 32, 33])
+@pytest.mark.parametrize("ahead", [0, 3])
+def test_cross_longest_sources_first(ops, dtype, portions, ahead):
+    """Two to 32 portions with more tiles than places for blocks: every tile of every request once, whatever the order of their sources; single tokens ahead, requests without a
+    token in between, tokens behind the last request.  (33 portions: the other side of the rule.)"""
+    rng = random.Random(portions)
+    new = [rng.choice([150, 257, 300]) if portions > 7 else 700 + 61 * i for i in range(portions)]
+    sources = {"unlike": [rng.choice([0, 1, 17, 64, 100, 333]) for _ in new], "alike": [90] * portions, "falling": [10 * (portions - i) for i in range(portions)],
+               "two lengths": [(40, 200)[i % 2] for i in range(portions)]}
+    for name, src in sources.items():
+        there = list(new)
+        if name in ("unlike", "two lengths") and portions > 2:
+            there[1] = there[portions // 2] = 0
+        counts, lens = [1] * ahead + there, [50, 0, 130][:ahead] + src
+        for spans in (None, spread_spans(counts, lens, portions)):
+            case = Case(dtype, 32, 32, 16, 16, counts, lens, spans, seed=portions, pad_rows=5)
+            assert (places(case) == "sources") == (portions <= 32)
+            case.check(ops)
+    case = Case(dtype, 16, 4, 64, 16, [1] * ahead + [x + 640 for x in new], [50, 0, 130][:ahead] + sources["unlike"], seed=portions, pad_rows=3)
+    assert (places(case) == "sources") == (portions <= 32)
+    case.check(ops)
+    ops.check_device_errors()
 
 
 # ---- heads with positions of several axes ----------------------------------------------------------------------------------------
