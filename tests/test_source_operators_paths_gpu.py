@@ -169,6 +169,18 @@ def test_cross_longest_sources_first(ops, dtype, portions, ahead):
     ops.check_device_errors()
 
 
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("R,K,chunks,sources", [(64, 8, 1, (2047, 2048, 2049, 4100, 6200)), (130, 4, 1, (2047, 2048, 2049, 4100)), (50, 6, 2, (4000, 4097, 4300, 5000)),
+                                                (37, 5, 4, (8193, 8300, 40)), (2, 2, 8, (17001, 18432))])
+def test_cross_single_tokens_over_long_sources(ops, page, R, K, chunks, sources):
+    """Runs of more than 32 stages of 16 positions a warp: where a warp's pages are looked up again.  One to eight blocks a request and kv head; spans that begin inside a stage."""
+    src = [sources[i % len(sources)] for i in range(R)]
+    assert ops.cross_decode_chunks(R * K, max(src)) == chunks and max(src) > 32 * 64 * chunks
+    Case(torch.bfloat16, 2 * K, K, 16, page, [1] * R, src, seed=R).check(ops)
+    spans = [[(5, s), (s // 3 + 7, s - 9), (0, s), (s - 2050, s + 10), (100, 2148 + i)][i % 5] for i, s in enumerate(src)]
+    Case(torch.bfloat16, 2 * K, K, 16, page, [1] * R, src, spans, seed=R + 1, pad_rows=1).check(ops)
+
+
 # ---- heads with positions of several axes ----------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", DTYPES)
