@@ -193,3 +193,43 @@ def test_axes_single_row_in_place(ops, dtype, stride):
     want, _, _ = axes_want(rows, weight, None, 1e-6, positions, axis_of, inv_freq, 64, False, 4, 0, 64)
     ops.qk_norm_axes_write(rows, rows, weight, None, 1e-6, positions, axis_of, inv_freq, 64, False, None, None, None, 4, 0, 64, write_kv=False)
     torch.testing.assert_close(rows.double(), want.reshape(1, -1), **axes_tolerance(dtype))
+
+
+LONG_AXES = [(32, 8, 128, 128, 16, 8007), (32, 8, 128, 128, 16, 2501), (16, 16, 80, 80, 16, 2501), (40, 8, 128, 64, 32, 1000), (96, 8, 128, 128, 16, 1501), (0, 1, 512, 512, 16, 1000),
+             (0, 1, 256, 256, 16, 1000), (14, 2, 96, 96, 64, 2501), (4, 2, 40, 20, 4, 1000), (1, 1, 24, 16, 16, 2501)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("H,K,d,rotary,page,T", LONG_AXES)
+def test_axes_many_tokens(ops, dtype, interleaved, H, K, d, rotary, page, T):
+    """Prompts of which every block takes several tokens, one after the other: rows that are on their way ahead, angles and places of groups of tokens in two buffers, a last group and a
+    last block that are not full; one part of the heads and several, fewer threads than a head has angles."""
+    for axes, norm, wide in ((3, True, 0), (1, False, 8)):
+        g = torch.Generator(device=DEV).manual_seed(T + axes)
+        half = rotary // 2
+        rows = torch.randn(T, (H + 2 * K) * d + wide, generator=g, device=DEV).to(dtype)[:, :(H + 2 * K) * d]
+        qw, kw = ((1 + 0.3 * torch.randn(d, generator=g, device=DEV)) if norm else None for _ in range(2))
+        axis_of = torch.randint(0, axes, (half,), generator=g, device=DEV).int()
+        inv_freq = torch.pow(10000.0, -2.0 * torch.arange(half, device=DEV) / rotary).float()
+        positions = torch.randint(0, 50000, (axes, T), generator=g, device=DEV).int()
+        pages = -(-T // page) + 2
+        slots = torch.randperm(pages * page, generator=g, device=DEV)[:T].int()
+        slots[torch.randperm(T, generator=g, device=DEV)[:T // 7]] = -1                     # padded tokens inside the runs
+        slots[T // 2] = pages * page                                                          # no place of the cache
+        k, v = (torch.full((pages, K, page, d), 9.0, device=DEV, dtype=dtype) for _ in range(2))
+        q_out = torch.empty(T, H * d, device=DEV, dtype=dtype) if H else None
+        ops.qk_norm_axes_write(rows, q_out, qw, kw, 1e-6, positions, axis_of, inv_freq, rotary, interleaved, slots, k, v, H, K, d)
+        q_want, k_want, v_want = axes_want(rows, qw, kw, 1e-6, positions, axis_of, inv_freq, rotary, interleaved, H, K, d)
+        k_ref, v_ref = (torch.full((pages, K, page, d), 9.0, device=DEV, dtype=torch.float64) for _ in range(2))
+        stored = (slots >= 0) & (slots < pages * page)
+        at = slots[stored].long()
+        k_ref[at // page, :, at % page], v_ref[at // page, :, at % page] = k_want[stored], v_want[stored]
+        if H:
+            torch.testing.assert_close(q_out.double(), q_want.reshape(T, H * d), **axes_tolerance(dtype))
+        torch.testing.assert_close(k.double(), k_ref, **axes_tolerance(dtype))
+        assert torch.equal(v.double(), v_ref)
+        if H:                                                        # queries alone, where they lie
+            lie = rows[:, :H * d].contiguous()
+            ops.qk_norm_axes_write(lie, lie, qw, None, 1e-6, positions, axis_of, inv_freq, rotary, interleaved, None, None, None, H, 0, d, write_kv=False)
+            assert torch.equal(lie, q_out)
