@@ -2984,21 +2984,23 @@ def cross_decode_supported(dtype, H: int, K: int, d: int, page_size: int) -> boo
     return dtype is torch.bfloat16 and d % 16 == 0 and 16 <= d <= 128 and H // K <= 8 and page_size >= 16
 
 
+def _cross_job(which: str, d: int) -> tuple:
+    return f"mb_attention_cross_{which}_d{d}", ([f"attention_cross_{which}.cu"], [f"HEAD_DIM={d}"])
+
+
 def cross_jobs(dtype, H: int, K: int, d: int, page_size: int) -> dict:
-    """``{library: (sources, defines)}`` of the kernels that ``attention_cross`` runs for this head layout."""
-    jobs = {"mb_attention_cross": (build.LIBRARIES["mb_attention_cross"], [])}
-    if cross_tc_supported(dtype, H, K, d, page_size):
-        jobs[f"mb_attention_cross_tc_d{d}"] = (["attention_cross_tc.cu"], [f"HEAD_DIM={d}"])
-    if cross_decode_supported(dtype, H, K, d, page_size):
-        jobs[f"mb_attention_cross_decode_d{d}"] = (["attention_cross_decode.cu"], [f"HEAD_DIM={d}"])
+    """``{library: (sources, defines)}`` of the kernels that ``attention_cross`` runs for this head layout: what a part that calls it adds to its ``kernel_jobs``
+    (``build.build_many`` compiles them; what is not there by then is compiled by the first call)."""
+    jobs = library_jobs("mb_attention_cross")
+    jobs.update(_cross_job(which, d) for which, supported in (("tc", cross_tc_supported), ("decode", cross_decode_supported)) if supported(dtype, H, K, d, page_size))
     return jobs
 
 
 def _cross_lib(which: str, d: int):
-    name = f"mb_attention_cross_{which}_d{d}"
+    name, (sources, defines) = _cross_job(which, d)
     lib = _libraries.get(name)
     if lib is None:
-        lib = _libraries[name] = build.load(name, [f"attention_cross_{which}.cu"], [f"HEAD_DIM={d}"])
+        lib = _libraries[name] = build.load(name, sources, defines)
     return lib
 
 
@@ -3018,7 +3020,9 @@ def attention_cross(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``p = softmax_j(scale * q[t, h] . k[j])`` over the source's positions, or with ``spans`` (int32 ``[T, 2]``) over those from ``spans[t, 0]`` up to but not
     including ``spans[t, 1]``; a token that sees nothing gets zeros.  Keys and values lie in pages ``[page, K, page_size, d]`` (a power of two of positions).  Of ``ctx`` it
     takes ``num_requests``, ``num_decode`` (the first requests, one token each), ``max_query_len`` and ``cu_tokens``; rows of ``q`` ``[T, H * d]`` past the last request's
-    are not read and those of ``out`` stay as they were, and so does the row of a request without a token (a padded batch's).  ``q`` may be columns of wider rows; ``out`` must not lie over it."""
+    are not read and those of ``out`` stay as they were, and so does the row of a request without a token (a padded batch's).  ``q`` may be columns of wider rows; ``out`` must not lie over it.
+    A head size's kernels are compiled by its first call where ``cross_jobs`` has not been built.  The tensor cores' waits are bounded: where one gives up its tile
+    has no results, and ``check_device_errors`` raises."""
     table, lens, cu = source.block_table, source.lens, ctx.cu_tokens
     device = q.get_device()
     if device < 0 or device != _current_device() or not device == k_cache.get_device() == v_cache.get_device() == out.get_device():
