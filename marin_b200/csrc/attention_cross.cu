@@ -17,6 +17,7 @@
 #define MB_LIB "attention_cross"
 #define MB_LIB_ID 42
 #include "cross_common.cuh"
+#include "mma_helpers.cuh"
 #include "pair_math.cuh"
 
 #define CX_BN 64
@@ -29,12 +30,6 @@ __host__ __device__ __forceinline__ int cross_chunks(int len) {
     while (c < CX_CHUNKS && c * CX_CHUNK < len) c <<= 1;
     return c;
 }
-
-__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // Four elements of a row of d, from element c on, as float32 into shared memory; zeros where there is no row and past d.
 template <typename T>
