@@ -164,9 +164,9 @@ __global__ void __launch_bounds__(XT_THREADS, 2) attention_cross_tc_kernel(const
     uint64_t* q_full = bars;
     uint64_t* s_full = bars + 1;                                    // [buffer] scores are there
     uint64_t* p_full = bars + 3;                                    // [buffer] weights are there (four warps arrive)
-    uint64_t* o_done = bars + 5;                                    // [buffer] P V of the buffer's weights is done
-    uint64_t* drained = bars + 7;
-    uint64_t* k_full = bars + 8;                                    // [stage]
+    uint64_t* o_done = bars + 5;                                    // [block % 4] P V of the block's weights is done
+    uint64_t* drained = bars + 9;
+    uint64_t* k_full = bars + 10;                                   // [stage]
     uint64_t* k_free = k_full + XT_STAGES;
     uint64_t* v_full = k_free + XT_STAGES;
     uint64_t* v_free = v_full + XT_STAGES;
@@ -195,7 +195,8 @@ __global__ void __launch_bounds__(XT_THREADS, 2) attention_cross_tc_kernel(const
     if (warp == 4) {                                                // (the queries are asked for at once; the keys' range is not known yet)
         if (lane == 0) {
             mbar_init(q_full, 1); mbar_init(drained, 1);
-            for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1); }
+            for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); }
+            for (int i = 0; i < 4; ++i) mbar_init(&o_done[i], 1);
             for (int i = 0; i < XT_STAGES; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_free[i], 1); mbar_init(&v_full[i], 1); mbar_init(&v_free[i], 1); }
             *abort = 0;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -316,6 +317,10 @@ __global__ void __launch_bounds__(XT_THREADS, 2) attention_cross_tc_kernel(const
                 const bool more = i + 2 < blocks;
                 ok = warp_wait(&v_full[st], (i / XT_STAGES) & 1, abort, error_flag, 43);
                 if (ok && more) ok = warp_wait(&k_full[next % XT_STAGES], (next / XT_STAGES) & 1, abort, error_flag, 45);
+                // (The rows wait for few of o_done's phases, and a wait for a phase says nothing unless the one before it is known to be over; nothing orders the arrivals of two commits
+                // on two barriers.  So each phase is seen here, before this block's weights are, which come later anyway: whoever sees the scores of block i knows that P V of
+                // block i - 4 and of those ahead of it has arrived, and asks for i - 1 at the latest, four barriers in turn.)
+                if (ok && i >= 2) ok = warp_wait(&o_done[(i - 2) & 3], ((i - 2) >> 2) & 1, abort, error_flag, 47);
                 if (ok) ok = warp_wait(&p_full[i & 1], (i >> 1) & 1, abort, error_flag, 44);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -323,7 +328,7 @@ __global__ void __launch_bounds__(XT_THREADS, 2) attention_cross_tc_kernel(const
 #pragma unroll
                 for (int kk = 0; kk < XT_BN / 16; ++kk)
                     umma_bf16_tmem_a(tmem_o, tmem_s + (uint32_t)((i & 1) * XT_BN + kk * 8), vdesc + (uint32_t)(kk * (2048 >> 4)), idesc_pv, (i > 0 || kk > 0) ? 1u : 0u, elected);
-                umma_commit(&o_done[i & 1], elected);
+                umma_commit(&o_done[i & 3], elected);
                 umma_commit(&v_free[st], elected);
                 if (more) scores(i + 2);                            // (S goes where P lies: the tensor core takes an issuer's products in their order)
             }
@@ -349,12 +354,8 @@ __global__ void __launch_bounds__(XT_THREADS, 2) attention_cross_tc_kernel(const
             float s[XT_BN];
             tmem_ld32_async(s_col, s);
             tmem_ld32_async(s_col + 32, s + 32);
-            // (P V of the block before last is done, these scores came after it.  Its barrier's phase is seen all the same, each one by every warp: a wait for the next phase
-            // says nothing unless the one before is known to be over, and nothing orders the arrivals of two commits on two barriers.)
-            if (i >= 2) ok = warp_wait(&o_done[i & 1], ((i >> 1) - 1) & 1, abort, error_flag, 47);
             tmem_ld_wait(s);
             tmem_ld_wait(s + 32);
-            if (!ok) break;
             const int key0 = (block0 + i) * XT_BN, from = mask_from - key0, to = mask_to - key0;
             if (__any_sync(0xffffffffu, from > 0 || to < XT_BN)) {
 #pragma unroll
@@ -372,7 +373,7 @@ __global__ void __launch_bounds__(XT_THREADS, 2) attention_cross_tc_kernel(const
             if (__any_sync(0xffffffffu, raise)) {
                 if (raise) { corr = xt_exp2(m_used - m_true); m_used = m_true; }
                 if (i > 0) {                                        // (P V of the blocks ahead has to be done)
-                    ok = warp_wait(&o_done[(i - 1) & 1], ((i - 1) >> 1) & 1, abort, error_flag, 47);
+                    ok = warp_wait(&o_done[(i - 1) & 3], ((i - 1) >> 2) & 1, abort, error_flag, 47);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
@@ -412,7 +413,7 @@ __global__ void __launch_bounds__(XT_THREADS, 2) attention_cross_tc_kernel(const
             l_run = l_run * corr + (u0 + u1);
         }
         if (nblk == 0) warp_wait(q_full, 0, abort, error_flag, 42);     // (nothing to do in this block of a cluster: what was asked for has to land all the same)
-        if (ok && nblk > 0) ok = warp_wait(&o_done[(nblk - 1) & 1], ((nblk - 1) >> 1) & 1, abort, error_flag, 47);
+        if (ok && nblk > 0) ok = warp_wait(&o_done[(nblk - 1) & 3], ((nblk - 1) >> 2) & 1, abort, error_flag, 47);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         float* sO = (float*)smem + (size_t)tid * XT_OLD;
         if (cluster > 1) {
