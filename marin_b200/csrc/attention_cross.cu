@@ -9,11 +9,12 @@
 // shared memory in chunk order.  A row's arithmetic depends on its request's source and its range only, not on the batch, the portion or the tile: the same bits.
 // Bound by shared memory and by latency: for 16 multiply-add pairs twice, a thread asks for eight times 16 bytes, a warp's 512 bytes come at 128 a cycle, so the four warps of an SM
 // wait twice as long for them as their multiply-adds take; the rest are a tile's four barriers at 2 to 4 blocks an SM.  Five requests of 370 tokens in all, 16 heads of 64 over
-// 2,908 positions 73 us (105 with tiles of 64 rows, page lookups in the loads and idle blocks that wait for their cluster; 82 with the weights read one by one, in pairs,
+// 2,908 positions 74 us (105 with tiles of 64 rows, page lookups in the loads and idle blocks that wait for their cluster; 82 with the weights read one by one, in pairs,
 // instead of four at a time); four of 300 tokens, 32 heads of 128 over 600 positions 480 us, 25 TFLOP/s, where the scores' products take 155, the values' 100 and the copies 100
 // that the others do not cover.  Larger shares a thread (8 x 4, 8 x 8 sums) want registers that leave too few warps: 64 rows of 128 threads 78 and 567, of 256 threads 76 and 520,
 // of 64 threads 155 and 1,317; 32 rows of 64 threads 84 and 654; 2 x 8 sums (eight lanes a row) 90 and 568.  Rows copied whole by one thread each (cp.async.bulk) with two
 // barriers a tile instead of four 74 and 465, and 116 for 110 with one request of 300 tokens.
+// bfloat16 comes element by element through registers, not by cp.async: four of 300 tokens, 32 heads of 128 over 600 positions (pages of 8) 692 us, 480 in float32.
 #define MB_LIB "attention_cross"
 #define MB_LIB_ID 42
 #include "cross_common.cuh"
@@ -286,7 +287,7 @@ MB_API int mb_attention_cross(const CrossCall* c, cudaStream_t s) {
     const int whole = c->dtype == MB_F32 && a.d % 4 == 0 && (((uintptr_t)c->k_cache | (uintptr_t)c->v_cache) & 15) == 0;
     const int q_whole = c->dtype == MB_F32 && a.d % 4 == 0 && ((uintptr_t)c->q & 15) == 0 && c->q_stride % 4 == 0;
     // Few rows a request (single tokens): tiles of as few, for every row that is not there asks shared memory for keys and values all the same.  (Float32, tiles of 4 rows
-    // against tiles of 16: 8 single tokens over 2,000 positions, 16 heads of 64 48 and 92 us; 32 over 100 to 2,000 113 and 233; 32 over 600 positions,
+    // against tiles of 16: 8 single tokens over 2,000 positions, 16 heads of 64 49 and 92 us; 32 over 100 to 2,000 113 and 233; 32 over 600 positions,
     // 32 heads of 128 over 8 81 and 117; 8 over 577 positions of the latter 40 and 39.)
     const long long rows = (long long)c->max_query * a.G;
     const int bm = rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : 32;

@@ -10,7 +10,7 @@
 //               product at 16 bits of a weight, for no more products.  (Where a value is infinite the first alone count: what is left of a weight may be 0.)
 // Maximum, sum and O are float32; warps, then blocks (in shared memory, rank order), add up theirs scaled to the common maximum.
 // Positions outside the row's range are zeros in shared memory (asked for with no bytes), so what lies there does not matter.
-// Measured on B200: 64 requests of 500 to 4,100 positions, 8 kv heads of 128 (547 MB) 89 us, 6.1 TB/s, 94 % of the copy rate; one request of 577 positions 5 us, its chain of
+// Measured on B200: 64 requests of 500 to 4,100 positions, 8 kv heads of 128 (547 MB) 91 us, 6.0 TB/s, 91 % of the copy rate; one request of 577 positions 6 us in a graph, its chain of
 // dependent loads (lengths, pages, keys), products and the cluster's meeting.
 #define MB_LIB "attention_cross_decode"
 #define MB_LIB_ID 44

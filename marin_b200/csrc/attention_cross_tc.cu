@@ -12,7 +12,7 @@
 // one's barriers, first loads and last stores are time in which the other works.
 // Warps 0..3 are the rows, 4 loads Q and K, 5 loads V, 6 issues the products.  Sums, maxima and O are float32; P is rounded to
 // bfloat16 as the products' operand (its error, at most 2^-8 of a weight, is that of the rounding of the result; the sum takes the weights before it).
-// Measured on B200 (heads of 128, four prompts of 1,024 tokens of 32 heads over 4,096 positions, 275 GFLOP): 240 us (277 over
+// Measured on B200 (heads of 128, four prompts of 1,024 tokens of 32 heads over 4,096 positions, 275 GFLOP): 235 us (277 over
 // seconds, at the power limit's clock of 1.6 GHz).  What was tried: two tiles a block over the same
 // keys, one block an SM, with blocks of 128 keys (267 us) or 64 (262), with two threads a row (258 to 272), an issuer for both (274): slower, although a
 // key then comes for twice as many rows; blocks that stay and take tile after tile, loads ahead into the next (265); the special-function unit's exponentials by a

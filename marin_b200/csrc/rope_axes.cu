@@ -8,8 +8,8 @@
 // u + half / VEC) or two of the head's vectors (pairs side by side), so no value changes lanes.  Two blocks an SM take equal runs of tokens, all heads at once: weights stay
 // in registers, three tokens' rows are on their way (a block a token had its threads wait for each token's rows and angles: 73 us at the first size below), and an angle is
 // worked out once for all heads, a thread an angle, tokens ahead of its use (the 64-bit product and sincospif are as many instructions as a head's whole norm and rotation).
-// Measured on B200: 8,007 tokens of 32 + 2 x 8 heads of 128, bfloat16, norm, three axes (197 MB): 37 us, 5.3 TB/s, 82 % of the copy rate (issue slots 64 % busy);
-// 2,501 tokens of 16 + 2 x 16 heads of 80, float32, pairs side by side (77 MB): 17 us, 4.5 TB/s; eight tokens 3 us, a launch and two trips to memory.
+// Measured on B200: 8,007 tokens of 32 + 2 x 8 heads of 128, bfloat16, norm, three axes (197 MB): 37 us, 5.3 TB/s, 81 % of the copy rate (issue slots 64 % busy);
+// 2,501 tokens of 16 + 2 x 16 heads of 80, float32, pairs side by side (77 MB): 17 us, 4.4 TB/s; eight tokens 3 us, a launch and two trips to memory.
 #define MB_LIB "rope_axes"
 #define MB_LIB_ID 41
 #include "common.cuh"
@@ -245,7 +245,8 @@ __global__ void __launch_bounds__(512, 2) heads_axes_kernel(AxesRows p, int unit
     cp_async_wait<0>();
 }
 
-// Any head size, rotary width and alignment: a warp takes a head through shared memory.
+// Any head size, rotary width and alignment: a warp takes a head through shared memory, four of a token's heads at a time, so a token's chain of trips bounds it: 16 + 2 x 16 heads of 80
+// with 40 turning, bfloat16, halves apart, 8 tokens 17 us, 8,007 124 (3 and 33 by the kernel above with 80 turning).
 template <typename T>
 __global__ void __launch_bounds__(128) heads_axes_any_kernel(AxesRows p) {
     extern __shared__ float ax_tab[];
